@@ -135,6 +135,112 @@ int opl_attention_f16(const opl_half_t* q, const opl_half_t* k,
                       int sequence, int head_dim, int causal,
                       opl_stream_t stream);
 
+/* Decoding with a paged key-value cache (no counterpart in the reference,
+ * whose attention takes whole contiguous [B,H,S,D] tensors): rotary positions,
+ * appending to the cache, attention of one new token over it.  Tensors may
+ * have any strides (in elements) as long as head_dim is contiguous; head_dim
+ * is at most 256.  Addresses and strides that are multiples of 16 bytes take
+ * the widest loads.  Indices that the device reads (slots, block table,
+ * lengths) are checked there: a bad one is not followed, and its code is left
+ * in the watchdog word (opl_read_and_clear_watchdog): 0x6b01 slot past the
+ * cache, 0x6b02 block-table entry outside the cache, 0x6b03 length negative or
+ * past the sequence's row of the block table. */
+
+/* A rotary embedding.  Pair i of the rot_dim / 2 pairs (elements i and
+ * i + rot_dim / 2, or 2i and 2i + 1 when `adjacent`) is turned by
+ * positions[axis][token] * inv_freq[i]; the first sections[0] pairs belong to
+ * axis 0, the next sections[1] to axis 1, and so on (video: time, height,
+ * width).  `inverse` turns back: the transposed matrix, which is also the
+ * gradient of the rotation.  rot_dim is even and at most head_dim; elements
+ * past it are copied; 0 rotates nothing and needs no pointers.  Angles are
+ * formed in FP64, the rotation in FP32, and each result is rounded once. */
+typedef struct opl_rope_spec {
+  const int64_t* positions; /* device, [axes][tokens] */
+  const float* inv_freq;    /* device, [rot_dim / 2] */
+  int rot_dim;
+  int axes;                 /* 1 to 4 */
+  int sections[4];          /* sum over the axes: rot_dim / 2 */
+  int adjacent;
+  int inverse;
+} opl_rope_spec;
+
+/* Keys and values in pages: token i of page p for key-value head h starts at
+ * k + p * k_page + i * k_token + h * k_head (v alike). */
+typedef struct opl_kv_cache {
+  void* k;
+  void* v;
+  int64_t pages;
+  int page_size;
+  int kv_heads;
+  int head_dim;
+  int64_t k_page, k_token, k_head;
+  int64_t v_page, v_token, v_head;
+} opl_kv_cache;
+
+/* out[t][h] = rotated x[t][h], [tokens, heads, head_dim].  out is x itself
+ * (same strides) or does not overlap it. */
+int opl_rope_f32(const float* x, float* out, int tokens, int heads, int head_dim,
+                 int64_t x_token, int64_t x_head, int64_t out_token, int64_t out_head,
+                 const opl_rope_spec* rope, opl_stream_t stream);
+int opl_rope_f16(const opl_half_t* x, opl_half_t* out, int tokens, int heads, int head_dim,
+                 int64_t x_token, int64_t x_head, int64_t out_token, int64_t out_head,
+                 const opl_rope_spec* rope, opl_stream_t stream);
+int opl_rope_bf16(const opl_bf16_t* x, opl_bf16_t* out, int tokens, int heads, int head_dim,
+                  int64_t x_token, int64_t x_head, int64_t out_token, int64_t out_head,
+                  const opl_rope_spec* rope, opl_stream_t stream);
+
+/* Rotates the new tokens' queries into q_out and their keys into the cache,
+ * and copies their values there: token t goes to token slots[t] % page_size
+ * of page slots[t] / page_size.  A negative slot keeps the token out of the
+ * cache (padding; its query is rotated all the same).  The slots that are not
+ * negative have to be distinct: of two tokens with the same slot either may
+ * win, element by element.  Nothing else of the cache is touched.  q is
+ * [tokens, heads, head_dim]; k and v are [tokens, kv_heads, head_dim]; q_out
+ * is q itself or overlaps nothing. */
+int opl_kv_append_f32(const float* q, int64_t q_token, int64_t q_head, const float* k,
+                      int64_t k_token, int64_t k_head, const float* v, int64_t v_token,
+                      int64_t v_head, float* q_out, int64_t out_token, int64_t out_head,
+                      const opl_kv_cache* cache, const int64_t* slots, int tokens, int heads,
+                      const opl_rope_spec* rope, opl_stream_t stream);
+int opl_kv_append_f16(const opl_half_t* q, int64_t q_token, int64_t q_head, const opl_half_t* k,
+                      int64_t k_token, int64_t k_head, const opl_half_t* v, int64_t v_token,
+                      int64_t v_head, opl_half_t* q_out, int64_t out_token, int64_t out_head,
+                      const opl_kv_cache* cache, const int64_t* slots, int tokens, int heads,
+                      const opl_rope_spec* rope, opl_stream_t stream);
+int opl_kv_append_bf16(const opl_bf16_t* q, int64_t q_token, int64_t q_head, const opl_bf16_t* k,
+                       int64_t k_token, int64_t k_head, const opl_bf16_t* v, int64_t v_token,
+                       int64_t v_head, opl_bf16_t* q_out, int64_t out_token, int64_t out_head,
+                       const opl_kv_cache* cache, const int64_t* slots, int tokens, int heads,
+                       const opl_rope_spec* rope, opl_stream_t stream);
+
+/* Attention of one new token per sequence: q and out are [batch, heads,
+ * head_dim] (out contiguous), query head h reads key-value head
+ * h / (heads / kv_heads), and sequence b has seq_lens[b] keys, key j in page
+ * block_table[b * table_row + j / page_size].  Softmax over scale * q.K in
+ * FP32; the result is rounded once to the tensors' type.  A sequence of length
+ * 0 gives zeros.  Table entries past a sequence's pages are not read, and
+ * neither are a page's tokens past its length.  Keys of a page outside the
+ * cache are left out.
+ * `workspace` is 16-byte aligned device memory of at least the size that
+ * opl_paged_attention_workspace gives; its contents do not matter and need not
+ * be kept, but two calls that may overlap on the GPU need one each. */
+int opl_paged_attention_workspace(int heads, int kv_heads, int head_dim, size_t* bytes);
+int opl_paged_attention_f32(const float* q, int64_t q_batch, int64_t q_head,
+                            const opl_kv_cache* cache, const int* block_table, int64_t table_row,
+                            int max_pages, const int* seq_lens, float* out, int batch, int heads,
+                            float scale, void* workspace, size_t workspace_bytes,
+                            opl_stream_t stream);
+int opl_paged_attention_f16(const opl_half_t* q, int64_t q_batch, int64_t q_head,
+                            const opl_kv_cache* cache, const int* block_table, int64_t table_row,
+                            int max_pages, const int* seq_lens, opl_half_t* out, int batch,
+                            int heads, float scale, void* workspace, size_t workspace_bytes,
+                            opl_stream_t stream);
+int opl_paged_attention_bf16(const opl_bf16_t* q, int64_t q_batch, int64_t q_head,
+                             const opl_kv_cache* cache, const int* block_table, int64_t table_row,
+                             int max_pages, const int* seq_lens, opl_bf16_t* out, int batch,
+                             int heads, float scale, void* workspace, size_t workspace_bytes,
+                             opl_stream_t stream);
+
 /* Library utilities (no reference counterpart). */
 
 /* cudaGetErrorString of an error code returned above. */

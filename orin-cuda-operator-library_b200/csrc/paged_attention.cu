@@ -1,0 +1,513 @@
+// Attention of one new token per sequence over a paged key-value cache
+// (opl_paged_attention_*), FP32 arithmetic, any head size up to 256, any
+// grouping of query heads, any strides with a unit last one.
+//
+//   out[b, h] = sum_j p_j V_j,  p_j = exp(s_j - max s) / sum_i exp(s_i - max s),
+//   s_j = scale * q[b, h] . K_j,  j < seq_lens[b], keys through the block table.
+//
+// This file has the SIMT kernel, which runs FP32 caches and every 16-bit
+// cache that the tensor-core kernel does not take, the launch that joins the
+// parts of units cut between CTAs, and the entry points.
+//
+// SIMT kernel.  The 32 lanes of a warp share a key: lane l holds E elements
+// of the queries (up to 8 rows), of the key, of the value and of the output.
+// A warp takes 8 keys at a time: E products a lane, row and key; the 8 x rows
+// sums over 32 lanes by a transposing butterfly (about one shuffle a sum
+// instead of five); one exponential a key and row; running maximum and sum
+// (log2 domain) and the output in registers.  The warps of a CTA take the
+// tiles of a segment in turn and merge through shared memory at its end.
+#include "paged_attention.cuh"
+
+namespace opl {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kTile = 8;  // keys of a warp's step
+constexpr int kLeast = kWarps;
+
+template <typename T>
+__device__ __forceinline__ float ld_f32(const T* p);
+template <>
+__device__ __forceinline__ float ld_f32(const float* p) {
+  return ld_stream(p);
+}
+template <>
+__device__ __forceinline__ float ld_f32(const __half* p) {
+  unsigned short b;
+  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(b) : "l"(p));
+  return __half2float(__ushort_as_half(b));
+}
+template <>
+__device__ __forceinline__ float ld_f32(const __nv_bfloat16* p) {
+  unsigned short b;
+  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(b) : "l"(p));
+  return __bfloat162float(__ushort_as_bfloat16(b));
+}
+
+__device__ __forceinline__ void st_out(float* p, float x) { *p = x; }
+__device__ __forceinline__ void st_out(__half* p, float x) { *p = __float2half_rn(x); }
+__device__ __forceinline__ void st_out(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+
+// Element e of a lane is element `column` of the head: vectors of up to four
+// consecutive floats when kVec, else every 32nd element.
+template <int E, bool kVec>
+__device__ __forceinline__ int column(int lane, int e) {
+  if (!kVec) return lane + 32 * e;
+  constexpr int kWidth = E < 4 ? E : 4;
+  return lane * kWidth + (e / kWidth) * 32 * kWidth + e % kWidth;
+}
+
+// A row of a head into the lane's E registers, zero past `dim` and where the
+// row is not there.
+template <typename T, int E, bool kVec>
+__device__ __forceinline__ void load_row(const T* row, int dim, int lane, float (&x)[E]) {
+  if constexpr (kVec) {
+    constexpr int kWidth = E < 4 ? E : 4;
+#pragma unroll
+    for (int c = 0; c < E; c += kWidth) {
+      const int d = column<E, kVec>(lane, c);
+      const bool there = row != nullptr && d < dim;
+      if constexpr (kWidth == 4) {
+        const float4 w = there ? ld_stream(reinterpret_cast<const float4*>(row + d))
+                               : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[c] = w.x, x[c + 1] = w.y, x[c + 2] = w.z, x[c + 3] = w.w;
+      } else {
+        float2 w = make_float2(0.f, 0.f);
+        if (there)
+          asm volatile("ld.global.nc.L1::no_allocate.v2.f32 {%0,%1}, [%2];"
+                       : "=f"(w.x), "=f"(w.y)
+                       : "l"(row + d));
+        x[c] = w.x, x[c + 1] = w.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int d = column<E, kVec>(lane, e);
+      x[e] = row != nullptr && d < dim ? ld_f32(row + d) : 0.0f;
+    }
+  }
+}
+
+// Sums v[i] over the warp for each of kCount values (a power of two, 8 to
+// 64).  Afterwards v[0] (and v[1] for 64) of lane l is the sum of value
+// index_of(l) (+ 1).
+template <int kCount>
+__device__ __forceinline__ void transpose_sum(float (&v)[kCount], int lane) {
+  int count = kCount;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (count > 1) {
+      count >>= 1;
+#pragma unroll
+      for (int i = 0; i < kCount / 2; ++i) {
+        if (i >= count) continue;
+        const bool upper = (lane & o) != 0;
+        const float give = upper ? v[i] : v[i + count];
+        const float keep = upper ? v[i + count] : v[i];
+        v[i] = keep + __shfl_xor_sync(kFullMask, give, o);
+      }
+    } else {
+      v[0] += __shfl_xor_sync(kFullMask, v[0], o);
+    }
+  }
+}
+
+constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
+
+template <typename T, int kRows, int E, bool kVec>
+__global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a, int row_cap) {
+  constexpr int kSums = kTile * kRows;  // value index: row * kTile + key
+  constexpr int kHeld = kSums > 32 ? kSums / 32 : 1;
+  constexpr int kWidth = 32 * E;
+  __shared__ float weights[kWarps][kRows][kTile];
+  __shared__ float rescale[kWarps][kRows];
+  __shared__ float merge_m[kWarps][kRows], merge_l[kWarps][kRows];
+  extern __shared__ float merge_o[];  // [kWarps][kRows][kWidth]
+  pdl_begin();
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const T* q = static_cast<const T*>(a.q);
+  const T* keys = static_cast<const T*>(a.k);
+  const T* values = static_cast<const T*>(a.v);
+  const int page_size = static_cast<int>(a.page_size.divisor);
+  const PagedStart start = paged_start<kThreads, kTile, kLeast>(
+      a, gridDim.x, [](long long total, int ctas) -> long long {
+        return static_cast<int>(blockIdx.x) < ctas ? range_begin(total, ctas, blockIdx.x) : -1;
+      });
+  if (static_cast<int>(blockIdx.x) >= start.ctas) return;
+  int64_t w = range_begin(start.total, start.ctas, blockIdx.x);
+  const int64_t limit = range_begin(start.total, start.ctas, blockIdx.x + 1);
+  int sequence = start.sequence;
+  int64_t before = start.before;
+  int reported = 0;
+
+  // Which row's score this lane holds after transpose_sum: the value index is
+  // spelled by the lane's bits from the top.
+  constexpr int kLogSums = log2_of(kSums);
+  const int index = kLogSums >= 5 ? lane << (kLogSums - 5) : lane >> (5 - kLogSums);
+  const int my_row = index / kTile, my_key = index % kTile;
+
+  while (w < limit) {
+    const int raw_length = ld_int(a.seq_lens + sequence);
+    const int length = readable_length(raw_length, a.max_pages, page_size);
+    if (length != raw_length) reported = kBadLength;
+    const int tiles = key_tiles(length, kTile);
+    if (w >= (before + tiles) * a.units()) {
+      before += tiles;
+      ++sequence;
+      continue;
+    }
+    const Segment segment = segment_at(w, limit, before, tiles, a.units());
+    w += segment.end - segment.begin;
+    const PagedUnit unit = paged_unit<kRows>(a, segment.unit);
+    const int* table = a.block_table + sequence * a.table_row;
+    const T* k_head = keys + unit.kv_head * a.k_head;
+    const T* v_head = values + unit.kv_head * a.v_head;
+
+    float qr[kRows][E], o[kRows][E];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      load_row<T, E, kVec>(r < unit.rows ? q + sequence * a.q_batch +
+                                               (unit.first_head + r) * a.q_head
+                                         : nullptr,
+                           a.head_dim, lane, qr[r]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[r][e] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;  // of my_row; l over my keys only
+
+    for (int tile = segment.begin + warp; tile < segment.end; tile += kWarps) {
+      const int base = tile * kTile;
+      // Lanes 0-7 place the tile's keys, lanes 8-15 its values.
+      int64_t place = -1;
+      {
+        const int key = base + (lane & 7);
+        if (lane < 16 && key < length) {
+          const int index_in_row = static_cast<int>(fast_div(key, a.page_size));
+          const int page = ld_int(table + index_in_row);
+          const int inside = key - index_in_row * page_size;
+          if (cache_page(page, a.pages))
+            place = lane < 8 ? page * a.k_page + inside * a.k_token
+                             : page * a.v_page + inside * a.v_token;
+          else
+            reported = kBadPage;
+        }
+      }
+      float kr[kTile][E], vr[kTile][E];
+      int64_t k_place[kTile];
+#pragma unroll
+      for (int j = 0; j < kTile; ++j) {
+        k_place[j] = __shfl_sync(kFullMask, place, j);
+        const int64_t v_place = __shfl_sync(kFullMask, place, 8 + j);
+        load_row<T, E, kVec>(k_place[j] >= 0 ? k_head + k_place[j] : nullptr, a.head_dim, lane,
+                             kr[j]);
+        load_row<T, E, kVec>(v_place >= 0 ? v_head + v_place : nullptr, a.head_dim, lane, vr[j]);
+      }
+      float s[kSums];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int j = 0; j < kTile; ++j) {
+          float dot = 0.0f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) dot = fmaf(qr[r][e], kr[j][e], dot);
+          s[r * kTile + j] = dot;
+        }
+      transpose_sum(s, lane);
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const bool there = __shfl_sync(kFullMask, place, my_key + i) >= 0;
+        s[i] = there ? s[i] * a.scale_log2 : -INFINITY;
+        top = fmaxf(top, s[i]);
+      }
+      // The lanes that hold one row differ in these bits.
+      constexpr int kRowLanes = kRows >= 4 ? 32 / kRows : 8;
+      constexpr int kFirst = kRows >= 4 ? 1 : 4 / kRows;
+#pragma unroll
+      for (int x = 1; x < kRowLanes; x <<= 1)
+        top = fmaxf(top, __shfl_xor_sync(kFullMask, top, x * kFirst));
+      const float m_new = fmaxf(m, top);
+      const float base_m = m_new == -INFINITY ? 0.0f : m_new;  // no key so far: all weights 0
+      const float alpha = paged_exp2(m - base_m);
+      __syncwarp();  // the previous tile's weights have been read
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const float p = paged_exp2(s[i] - base_m);
+        weights[warp][my_row][my_key + i] = p;
+        sum += p;
+      }
+      if (my_key == 0) rescale[warp][my_row] = alpha;
+      l = l * alpha + sum;
+      m = m_new;
+      __syncwarp();
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const float alpha_r = rescale[warp][r];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[r][e] *= alpha_r;
+#pragma unroll
+        for (int j = 0; j < kTile; ++j) {
+          const float p = weights[warp][r][j];
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[r][e] = fmaf(p, vr[j][e], o[r][e]);
+        }
+      }
+    }
+
+    // Merge the warps: every lane that holds a row has its maximum; the sum
+    // is over the lanes (and, where several lanes hold the same key, one of
+    // them).
+    float l_row = l;
+    constexpr int kRowLanes = kRows >= 4 ? 32 / kRows : 8;
+    constexpr int kFirst = kRows >= 4 ? 1 : 4 / kRows;
+#pragma unroll
+    for (int x = 1; x < kRowLanes; x <<= 1)
+      l_row += __shfl_xor_sync(kFullMask, l_row, x * kFirst);
+    if (my_key == 0) {
+      merge_m[warp][my_row] = m;
+      merge_l[warp][my_row] = l_row;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        merge_o[(warp * kRows + r) * kWidth + column<E, kVec>(lane, e)] = o[r][e];
+    __syncthreads();
+    const int slot = 2 * blockIdx.x + segment.slot();
+    for (int i = threadIdx.x; i < unit.rows * a.head_dim; i += kThreads) {
+      const int r = i / a.head_dim, d = i - r * a.head_dim;
+      float top = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) top = fmaxf(top, merge_m[x][r]);
+      const float base_m = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f, out = 0.0f;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) {
+        const float f = paged_exp2(merge_m[x][r] - base_m);
+        sum = fmaf(f, merge_l[x][r], sum);
+        out = fmaf(f, merge_o[(x * kRows + r) * kWidth + d], out);
+      }
+      if (segment.whole()) {
+        st_out(static_cast<T*>(a.out) +
+                   (static_cast<int64_t>(sequence) * a.heads + unit.first_head + r) * a.head_dim + d,
+               length == 0 ? 0.0f : out / sum);
+      } else {
+        const int64_t row = static_cast<int64_t>(slot) * row_cap + r;
+        a.partial[row * a.head_dim + d] = out;
+        if (d == 0) a.partial_ml[row] = make_float2(top, sum);
+      }
+    }
+    __syncthreads();
+  }
+  if (reported != 0) watchdog_trip(a.watchdog, reported);
+}
+
+// Joins the parts of the unit that CTA blockIdx.x of the main launch starts
+// and does not end (slot 1 of that CTA, slot 0 of the following ones), row
+// blockIdx.y, in key order.
+template <typename T, int kUnitTile, int kUnitLeast, int kRows>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int grid_ctas,
+                                                         int row_cap) {
+  __shared__ float top_of_warp[4];
+  pdl_begin();
+  int64_t at = 0, limit = 0;
+  const int cta = blockIdx.x;
+  const PagedStart start = paged_start<128, kUnitTile, kUnitLeast>(
+      a, grid_ctas, [&](long long total, int ctas) -> long long {
+        if (cta + 1 >= ctas) return -1;
+        limit = range_begin(total, ctas, cta + 1);
+        at = limit - 1;  // the last tile of the CTA
+        return at;
+      });
+  if (cta + 1 >= start.ctas) return;
+  const int sequence = start.sequence;
+  const int length = paged_length(a, sequence);
+  const int tiles = key_tiles(length, kUnitTile);
+  const Segment last = segment_at(at, limit, start.before, tiles, a.units());
+  if (last.end == tiles) return;  // not cut here
+  const int64_t unit_begin = at - last.begin;
+  if (unit_begin < range_begin(start.total, start.ctas, cta)) return;  // an earlier CTA starts it
+  const PagedUnit unit = paged_unit<kRows>(a, last.unit);
+  const int row = blockIdx.y;
+  if (row >= unit.rows) return;
+  const int end_cta = range_owner(start.total, start.ctas, unit_begin + tiles - 1);
+  const int parts = end_cta - cta + 1;
+  const auto part_row = [&](int p) {
+    const int slot = p == 0 ? 2 * cta + 1 : 2 * (cta + p);
+    return static_cast<int64_t>(slot) * row_cap + row;
+  };
+  float top = -INFINITY;
+  for (int p = threadIdx.x; p < parts; p += 128) top = fmaxf(top, __ldcg(&a.partial_ml[part_row(p)]).x);
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) top_of_warp[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(top_of_warp[0], top_of_warp[1]), fmaxf(top_of_warp[2], top_of_warp[3]));
+  const float base_m = top == -INFINITY ? 0.0f : top;
+  for (int d = threadIdx.x; d < a.head_dim; d += 128) {
+    float sum = 0.0f, out = 0.0f;
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+      const float2 ml = __ldcg(&a.partial_ml[part_row(p)]);
+      const float f = paged_exp2(ml.x - base_m);
+      sum = fmaf(f, ml.y, sum);
+      out = fmaf(f, __ldcg(&a.partial[part_row(p) * a.head_dim + d]), out);
+    }
+    st_out(static_cast<T*>(a.out) +
+               (static_cast<int64_t>(sequence) * a.heads + unit.first_head + row) * a.head_dim + d,
+           out / sum);
+  }
+}
+
+template <typename T, int kRows, int E, bool kVec>
+int launch_simt(PagedArgs a, int grid_ctas, cudaStream_t stream) {
+  a.parts = (a.group + kRows - 1) / kRows;
+  const int row_cap = a.group < kRows ? a.group : kRows;
+  a.partial_ml = reinterpret_cast<float2*>(a.partial + static_cast<int64_t>(grid_ctas) * 2 *
+                                                           row_cap * a.head_dim);
+  constexpr size_t kShared = sizeof(float) * kWarps * kRows * 32 * E;
+  static_assert(kShared <= 40 * 1024, "fits without an opt-in");
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid_ctas);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = kShared;
+  config.stream = stream;
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  cudaError_t error = cudaLaunchKernelEx(&config, paged_simt_kernel<T, kRows, E, kVec>, a, row_cap);
+  if (error == cudaSuccess && grid_ctas > 1)
+    error = launch_pdl(paged_join_kernel<T, kTile, kLeast, kRows>, dim3(grid_ctas - 1, row_cap),
+                       dim3(128), stream, a, grid_ctas, row_cap);
+  return error != cudaSuccess ? error : cudaGetLastError();
+}
+
+template <typename T, int E, bool kVec>
+int pick_rows(const PagedArgs& a, int grid_ctas, cudaStream_t stream) {
+  if (a.group == 1) return launch_simt<T, 1, E, kVec>(a, grid_ctas, stream);
+  if (a.group == 2) return launch_simt<T, 2, E, kVec>(a, grid_ctas, stream);
+  // A lane holds rows * E elements of q and of the output each.
+  if (a.group <= 4 || E == 8) return launch_simt<T, 4, E, kVec>(a, grid_ctas, stream);
+  return launch_simt<T, 8, E == 8 ? 4 : E, kVec>(a, grid_ctas, stream);
+}
+
+bool aligned_rows(const PagedArgs& a, size_t element, int vector) {
+  const size_t bytes = element * vector;
+  const int64_t strides[] = {a.q_batch, a.q_head, a.k_page, a.k_token, a.k_head,
+                             a.v_page,  a.v_token, a.v_head, a.head_dim};
+  for (int64_t s : strides)
+    if (s % vector != 0) return false;
+  for (const void* p : {a.q, a.k, a.v})
+    if (reinterpret_cast<std::uintptr_t>(p) % bytes != 0) return false;
+  return true;
+}
+
+int grid_limit() { return 2 * sm_count(); }
+
+// CTAs of a launch: no more than the longest possible batch can use.
+int grid_for(const PagedArgs& a, int tile, int least, int unit_rows) {
+  const int64_t capacity = static_cast<int64_t>(a.max_pages) * a.page_size.divisor;
+  const int64_t tiles = capacity <= tile ? 1 : (capacity - 1) / tile + 1;
+  const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads *
+                        ((a.group + unit_rows - 1) / unit_rows);
+  const int limit = grid_limit();
+  // Saturates well below 2^63: only its comparison with the limit counts.
+  const double total = static_cast<double>(tiles) * static_cast<double>(units);
+  if (total >= static_cast<double>(limit) * least) return limit;
+  return active_ctas(tiles * units, limit, least);
+}
+
+template <typename T>
+int paged_attention(const void* q, int64_t q_batch, int64_t q_head, const opl_kv_cache* cache,
+                    const int* block_table, int64_t table_row, int max_pages, const int* seq_lens,
+                    void* out, int batch, int heads, float scale, void* workspace,
+                    size_t workspace_bytes, cudaStream_t stream) {
+  if (q == nullptr || cache == nullptr || cache->k == nullptr || cache->v == nullptr ||
+      block_table == nullptr || seq_lens == nullptr || out == nullptr || workspace == nullptr ||
+      batch <= 0 || heads <= 0 || max_pages <= 0 || cache->pages <= 0 || cache->page_size <= 0 ||
+      cache->kv_heads <= 0 || heads % cache->kv_heads != 0 || cache->head_dim <= 0 ||
+      cache->head_dim > kPagedMaxHeadDim || !(scale - scale == 0.0f) ||
+      reinterpret_cast<std::uintptr_t>(workspace) % 16 != 0)
+    return cudaErrorInvalidValue;
+  size_t needed = 0;
+  const int status = opl_paged_attention_workspace(heads, cache->kv_heads, cache->head_dim, &needed);
+  if (status != cudaSuccess) return status;
+  if (workspace_bytes < needed) return cudaErrorInvalidValue;
+  PagedArgs a = {};
+  a.q = q;
+  a.k = cache->k;
+  a.v = cache->v;
+  a.out = out;
+  a.q_batch = q_batch;
+  a.q_head = q_head;
+  a.k_page = cache->k_page;
+  a.k_token = cache->k_token;
+  a.k_head = cache->k_head;
+  a.v_page = cache->v_page;
+  a.v_token = cache->v_token;
+  a.v_head = cache->v_head;
+  a.block_table = block_table;
+  a.table_row = table_row;
+  a.seq_lens = seq_lens;
+  a.pages = cache->pages;
+  a.page_size = make_fast_div(cache->page_size);
+  a.max_pages = max_pages;
+  a.batch = batch;
+  a.heads = heads;
+  a.kv_heads = cache->kv_heads;
+  a.head_dim = cache->head_dim;
+  a.group = heads / cache->kv_heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.partial = static_cast<float*>(workspace);
+  a.watchdog = watchdog_word();
+  if (a.watchdog == nullptr) return cudaErrorInvalidDevice;
+  const bool vec = sizeof(T) == 4 && aligned_rows(a, sizeof(T), 4);
+  const int grid = grid_for(a, kTile, kLeast, a.group <= 4 ? a.group : 4);
+  if constexpr (sizeof(T) == 4) {
+    if (vec && a.head_dim <= 64) return pick_rows<T, 2, true>(a, grid, stream);
+    if (vec && a.head_dim <= 128) return pick_rows<T, 4, true>(a, grid, stream);
+    if (vec) return pick_rows<T, 8, true>(a, grid, stream);
+  }
+  if (a.group == 1) return launch_simt<T, 1, 8, false>(a, grid, stream);
+  return launch_simt<T, 4, 8, false>(a, grid, stream);
+}
+
+}  // namespace
+
+}  // namespace opl
+
+extern "C" {
+
+int opl_paged_attention_workspace(int heads, int kv_heads, int head_dim, size_t* bytes) {
+  if (bytes == nullptr || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 ||
+      head_dim > opl::kPagedMaxHeadDim)
+    return cudaErrorInvalidValue;
+  // Two partial units a CTA, up to 16 rows each, and their maxima and sums.
+  const size_t rows = heads / kv_heads < 16 ? heads / kv_heads : 16;
+  *bytes = static_cast<size_t>(opl::grid_limit()) * 2 * rows *
+           (sizeof(float) * static_cast<size_t>((head_dim + 1) / 2 * 2) + sizeof(float2));
+  return cudaSuccess;
+}
+
+#define OPL_PAGED_ENTRY(SUFFIX, ABI_T, T)                                                          \
+  int opl_paged_attention_##SUFFIX(const ABI_T* q, int64_t q_batch, int64_t q_head,                \
+                                   const opl_kv_cache* cache, const int* block_table,              \
+                                   int64_t table_row, int max_pages, const int* seq_lens,          \
+                                   ABI_T* out, int batch, int heads, float scale, void* workspace, \
+                                   size_t workspace_bytes, opl_stream_t stream) {                  \
+    return opl::paged_attention<T>(q, q_batch, q_head, cache, block_table, table_row, max_pages,   \
+                                   seq_lens, out, batch, heads, scale, workspace, workspace_bytes, \
+                                   stream);                                                        \
+  }
+
+OPL_PAGED_ENTRY(f32, float, float)
+OPL_PAGED_ENTRY(f16, opl_half_t, __half)
+OPL_PAGED_ENTRY(bf16, opl_bf16_t, __nv_bfloat16)
+
+}  // extern "C"

@@ -5,7 +5,9 @@ Two ways in, both onto the same compiled kernels in ``libopl_b200.so``:
 * ``load_operatorlib()`` registers ``torch.ops.operatorlib.{reduce_sum,
   softmax, transpose, rmsnorm, gemm, attention}`` -- the same schemas as the
   reference's TORCH_LIBRARY binding (python/operatorlib_binding.cpp:190-206)
-  and the same loader name as its python/load_extension.py:17.
+  and the same loader name as its python/load_extension.py:17 -- and
+  ``{rope, kv_append, paged_attention}``, decoding with a paged key-value
+  cache, which the reference does not have.
 * ``capi()`` returns the C-ABI (include/operatorlib/opl_capi.h) bound with
   ctypes; the raw-pointer helpers below call it with torch tensors' device
   pointers and the current stream, without going through the torch binding.
@@ -38,8 +40,29 @@ class OplError(RuntimeError):
         self.code = code
 
 
+class RopeSpec(ctypes.Structure):
+    """opl_rope_spec of the C-ABI."""
+
+    _fields_ = [("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+                ("rot_dim", ctypes.c_int), ("axes", ctypes.c_int),
+                ("sections", ctypes.c_int * 4), ("adjacent", ctypes.c_int),
+                ("inverse", ctypes.c_int)]
+
+
+class KvCache(ctypes.Structure):
+    """opl_kv_cache of the C-ABI."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("head_dim", ctypes.c_int)] + [
+        (name, ctypes.c_int64)
+        for name in ("k_page", "k_token", "k_head", "v_page", "v_token", "v_head")]
+
+
 def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     vp, i, sz, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
+    i64 = ctypes.c_int64
+    rope, cache = ctypes.POINTER(RopeSpec), ctypes.POINTER(KvCache)
     sigs = {
         "opl_reduce_sum_f32": [vp, vp, sz, vp],
         "opl_reduce_sum_partial_f64": [vp, vp, sz, vp],
@@ -56,7 +79,13 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
         "opl_attention_f32": [vp, vp, vp, vp, i, i, i, i, i, vp],
         "opl_attention_f16": [vp, vp, vp, vp, i, i, i, i, i, vp],
         "opl_read_and_clear_watchdog": [ctypes.POINTER(ctypes.c_int)],
+        "opl_paged_attention_workspace": [i, i, i, ctypes.POINTER(sz)],
     }
+    for suffix in ("f32", "f16", "bf16"):
+        sigs[f"opl_rope_{suffix}"] = [vp, vp, i, i, i, i64, i64, i64, i64, rope, vp]
+        sigs[f"opl_kv_append_{suffix}"] = [vp, i64, i64] * 4 + [cache, vp, i, i, rope, vp]
+        sigs[f"opl_paged_attention_{suffix}"] = [vp, i64, i64, cache, vp, i64, i, vp, vp, i, i,
+                                                 f, vp, sz, vp]
     for name, args in sigs.items():
         fn = getattr(lib, name)
         fn.argtypes = args
@@ -117,9 +146,13 @@ def version() -> str:
 from .raw import (  # noqa: E402  (re-exported convenience layer)
     attention_into,
     gemm_into,
+    kv_append_into,
+    paged_attention_into,
+    paged_attention_workspace,
     reduce_sum_into,
     reduce_sum_partial_f64_into,
     rmsnorm_into,
+    rope_into,
     softmax_into,
     transpose_into,
 )
@@ -128,8 +161,8 @@ from .team import ReduceTeam  # noqa: E402
 
 __all__ = [
     "ReduceTeam",
-    "OplError", "capi", "load_operatorlib", "check", "version",
-    "attention_into", "gemm_into", "reduce_sum_into",
-    "reduce_sum_partial_f64_into", "rmsnorm_into", "softmax_into",
-    "transpose_into",
+    "OplError", "KvCache", "RopeSpec", "capi", "load_operatorlib", "check", "version",
+    "attention_into", "gemm_into", "kv_append_into", "paged_attention_into",
+    "paged_attention_workspace", "reduce_sum_into", "reduce_sum_partial_f64_into",
+    "rmsnorm_into", "rope_into", "softmax_into", "transpose_into",
 ]

@@ -3,7 +3,9 @@
 Each ``*_into`` function takes contiguous CUDA tensors with preallocated
 outputs, passes their device pointers and the current CUDA stream (or
 ``stream``) to the matching ``opl_*`` entry point and raises ``OplError`` on a
-non-zero return -- the same contract a C, cgo or JNI caller gets.
+non-zero return -- the same contract a C, cgo or JNI caller gets.  The paged
+cache functions (``rope_into``, ``kv_append_into``, ``paged_attention_into``)
+take strided tensors whose last dimension is contiguous.
 """
 from __future__ import annotations
 
@@ -86,3 +88,95 @@ def attention_into(q, k, v, out, causal: bool, stream=None) -> None:
           else _lib().opl_attention_f32)
     _check("attention", fn(_ptr(q), _ptr(k), _ptr(v), _ptr(out), b, h, s, d,
                            int(bool(causal)), _stream(q, stream)))
+
+
+def _rope_spec(positions, inv_freq, sections, adjacent, inverse):
+    from . import RopeSpec
+
+    pairs = inv_freq.numel()
+    sections = list(sections) if sections else [pairs]
+    if len(sections) > 4:
+        raise ValueError("a rotary embedding has at most 4 position axes")
+    spec = RopeSpec(positions=_ptr(positions), inv_freq=_ptr(inv_freq), rot_dim=2 * pairs,
+                    axes=len(sections), adjacent=int(bool(adjacent)),
+                    inverse=int(bool(inverse)))
+    spec.sections[:len(sections)] = sections
+    return spec
+
+
+def _kv_cache(k_cache, v_cache):
+    from . import KvCache
+
+    pages, page_size, kv_heads, head_dim = k_cache.shape
+    return KvCache(_ptr(k_cache), _ptr(v_cache), pages, page_size, kv_heads, head_dim,
+                   *k_cache.stride()[:3], *v_cache.stride()[:3])
+
+
+def rope_into(x, out, positions, inv_freq, sections=None, adjacent=False, inverse=False,
+              stream=None) -> None:
+    """Rotary embedding of x [tokens, heads, head_dim] (FP32, FP16 or BF16)
+    into out, which may be x.  positions: int64 [tokens] or [axes, tokens],
+    contiguous; inv_freq: FP32 [rotated pairs]; sections: pairs of each axis."""
+    import ctypes
+
+    import torch
+
+    tokens, heads, head_dim = x.shape
+    spec = _rope_spec(positions, inv_freq, sections, adjacent, inverse)
+    with torch.cuda.device(x.device):
+        _check("rope", _dtype_fn("rope", x.dtype)(
+            _ptr(x), _ptr(out), tokens, heads, head_dim, *x.stride()[:2], *out.stride()[:2],
+            ctypes.byref(spec), _stream(x, stream)))
+
+
+def kv_append_into(q, k, v, q_out, k_cache, v_cache, slots, positions, inv_freq, sections=None,
+                   adjacent=False, stream=None) -> None:
+    """Rotates q into q_out (which may be q) and k into the cache, and copies v
+    there.  The caches are [pages, page_size, kv_heads, head_dim]; slots: int64
+    [tokens], contiguous, page * page_size + token of the page, negative for a
+    token that is not kept; the rest as in rope_into."""
+    import ctypes
+
+    import torch
+
+    spec = _rope_spec(positions, inv_freq, sections, adjacent, False)
+    cache = _kv_cache(k_cache, v_cache)
+    with torch.cuda.device(q.device):
+        _check("kv_append", _dtype_fn("kv_append", q.dtype)(
+            _ptr(q), *q.stride()[:2], _ptr(k), *k.stride()[:2], _ptr(v), *v.stride()[:2],
+            _ptr(q_out), *q_out.stride()[:2], ctypes.byref(cache), _ptr(slots), q.shape[0],
+            q.shape[1], ctypes.byref(spec), _stream(q, stream)))
+
+
+def paged_attention_workspace(heads: int, kv_heads: int, head_dim: int, device) -> "torch.Tensor":
+    """Scratch for paged_attention_into; calls that may overlap need one each."""
+    import ctypes
+
+    import torch
+
+    size = ctypes.c_size_t()
+    with torch.cuda.device(device):
+        _check("paged_attention", _lib().opl_paged_attention_workspace(
+            heads, kv_heads, head_dim, ctypes.byref(size)))
+        return torch.empty(size.value, dtype=torch.uint8, device=device)
+
+
+def paged_attention_into(q, k_cache, v_cache, block_table, seq_lens, out, workspace, scale=None,
+                         stream=None) -> None:
+    """Attention of q [batch, heads, head_dim], one new token per sequence,
+    over the cache (see kv_append_into) into the contiguous out.  block_table:
+    int32 [batch, pages of the longest sequence]; seq_lens: int32 [batch];
+    workspace from paged_attention_workspace; scale: 1 / sqrt(head_dim)."""
+    import ctypes
+
+    import torch
+
+    batch, heads, head_dim = q.shape
+    cache = _kv_cache(k_cache, v_cache)
+    scale = head_dim ** -0.5 if scale is None else float(scale)
+    with torch.cuda.device(q.device):
+        _check("paged_attention", _dtype_fn("paged_attention", q.dtype)(
+            _ptr(q), *q.stride()[:2], ctypes.byref(cache), _ptr(block_table),
+            block_table.stride(0), block_table.shape[1], _ptr(seq_lens), _ptr(out), batch, heads,
+            scale, _ptr(workspace), workspace.numel() * workspace.element_size(),
+            _stream(q, stream)))
