@@ -46,10 +46,6 @@ __device__ __forceinline__ float ld_f32(const __nv_bfloat16* p) {
   return __bfloat162float(__ushort_as_bfloat16(b));
 }
 
-__device__ __forceinline__ void st_out(float* p, float x) { *p = x; }
-__device__ __forceinline__ void st_out(__half* p, float x) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void st_out(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
-
 // Element e of a lane is element `column` of the head: vectors of up to four
 // consecutive floats when kVec, else every 32nd element.
 template <int E, bool kVec>
@@ -307,62 +303,6 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a,
   if (reported != 0) watchdog_trip(a.watchdog, reported);
 }
 
-// Joins the parts of the unit that CTA blockIdx.x of the main launch starts
-// and does not end (slot 1 of that CTA, slot 0 of the following ones), row
-// blockIdx.y, in key order.
-template <typename T, int kUnitTile, int kUnitLeast, int kRows>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int grid_ctas,
-                                                         int row_cap) {
-  __shared__ float top_of_warp[4];
-  pdl_begin();
-  int64_t at = 0, limit = 0;
-  const int cta = blockIdx.x;
-  const PagedStart start = paged_start<128, kUnitTile, kUnitLeast>(
-      a, grid_ctas, [&](long long total, int ctas) -> long long {
-        if (cta + 1 >= ctas) return -1;
-        limit = range_begin(total, ctas, cta + 1);
-        at = limit - 1;  // the last tile of the CTA
-        return at;
-      });
-  if (cta + 1 >= start.ctas) return;
-  const int sequence = start.sequence;
-  const int length = paged_length(a, sequence);
-  const int tiles = key_tiles(length, kUnitTile);
-  const Segment last = segment_at(at, limit, start.before, tiles, a.units());
-  if (last.end == tiles) return;  // not cut here
-  const int64_t unit_begin = at - last.begin;
-  if (unit_begin < range_begin(start.total, start.ctas, cta)) return;  // an earlier CTA starts it
-  const PagedUnit unit = paged_unit<kRows>(a, last.unit);
-  const int row = blockIdx.y;
-  if (row >= unit.rows) return;
-  const int end_cta = range_owner(start.total, start.ctas, unit_begin + tiles - 1);
-  const int parts = end_cta - cta + 1;
-  const auto part_row = [&](int p) {
-    const int slot = p == 0 ? 2 * cta + 1 : 2 * (cta + p);
-    return static_cast<int64_t>(slot) * row_cap + row;
-  };
-  float top = -INFINITY;
-  for (int p = threadIdx.x; p < parts; p += 128) top = fmaxf(top, __ldcg(&a.partial_ml[part_row(p)]).x);
-  top = warp_max(top);
-  if ((threadIdx.x & 31) == 0) top_of_warp[threadIdx.x >> 5] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(top_of_warp[0], top_of_warp[1]), fmaxf(top_of_warp[2], top_of_warp[3]));
-  const float base_m = top == -INFINITY ? 0.0f : top;
-  for (int d = threadIdx.x; d < a.head_dim; d += 128) {
-    float sum = 0.0f, out = 0.0f;
-#pragma unroll 4
-    for (int p = 0; p < parts; ++p) {
-      const float2 ml = __ldcg(&a.partial_ml[part_row(p)]);
-      const float f = paged_exp2(ml.x - base_m);
-      sum = fmaf(f, ml.y, sum);
-      out = fmaf(f, __ldcg(&a.partial[part_row(p) * a.head_dim + d]), out);
-    }
-    st_out(static_cast<T*>(a.out) +
-               (static_cast<int64_t>(sequence) * a.heads + unit.first_head + row) * a.head_dim + d,
-           out / sum);
-  }
-}
-
 template <typename T, int kRows, int E, bool kVec>
 int launch_simt(PagedArgs a, int grid_ctas, cudaStream_t stream) {
   a.parts = (a.group + kRows - 1) / kRows;
@@ -383,8 +323,7 @@ int launch_simt(PagedArgs a, int grid_ctas, cudaStream_t stream) {
   config.numAttrs = 1;
   cudaError_t error = cudaLaunchKernelEx(&config, paged_simt_kernel<T, kRows, E, kVec>, a, row_cap);
   if (error == cudaSuccess && grid_ctas > 1)
-    error = launch_pdl(paged_join_kernel<T, kTile, kLeast, kRows>, dim3(grid_ctas - 1, row_cap),
-                       dim3(128), stream, a, grid_ctas, row_cap);
+    error = launch_join<T, kTile, kLeast, kRows>(a, grid_ctas, row_cap, stream);
   return error != cudaSuccess ? error : cudaGetLastError();
 }
 
@@ -406,21 +345,6 @@ bool aligned_rows(const PagedArgs& a, size_t element, int vector) {
   for (const void* p : {a.q, a.k, a.v})
     if (reinterpret_cast<std::uintptr_t>(p) % bytes != 0) return false;
   return true;
-}
-
-int grid_limit() { return 2 * sm_count(); }
-
-// CTAs of a launch: no more than the longest possible batch can use.
-int grid_for(const PagedArgs& a, int tile, int least, int unit_rows) {
-  const int64_t capacity = static_cast<int64_t>(a.max_pages) * a.page_size.divisor;
-  const int64_t tiles = capacity <= tile ? 1 : (capacity - 1) / tile + 1;
-  const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads *
-                        ((a.group + unit_rows - 1) / unit_rows);
-  const int limit = grid_limit();
-  // Saturates well below 2^63: only its comparison with the limit counts.
-  const double total = static_cast<double>(tiles) * static_cast<double>(units);
-  if (total >= static_cast<double>(limit) * least) return limit;
-  return active_ctas(tiles * units, limit, least);
 }
 
 template <typename T>
@@ -468,7 +392,10 @@ int paged_attention(const void* q, int64_t q_batch, int64_t q_head, const opl_kv
   a.watchdog = watchdog_word();
   if (a.watchdog == nullptr) return cudaErrorInvalidDevice;
   const bool vec = sizeof(T) == 4 && aligned_rows(a, sizeof(T), 4);
-  const int grid = grid_for(a, kTile, kLeast, a.group <= 4 ? a.group : 4);
+  if constexpr (sizeof(T) == 2) {
+    if (aligned_rows(a, sizeof(T), 8)) return paged_attention_mma<T>(a, stream);
+  }
+  const int grid = paged_grid(a, paged_grid_limit(), kTile, kLeast, a.group <= 4 ? a.group : 4);
   if constexpr (sizeof(T) == 4) {
     if (vec && a.head_dim <= 64) return pick_rows<T, 2, true>(a, grid, stream);
     if (vec && a.head_dim <= 128) return pick_rows<T, 4, true>(a, grid, stream);
@@ -490,7 +417,7 @@ int opl_paged_attention_workspace(int heads, int kv_heads, int head_dim, size_t*
     return cudaErrorInvalidValue;
   // Two partial units a CTA, up to 16 rows each, and their maxima and sums.
   const size_t rows = heads / kv_heads < 16 ? heads / kv_heads : 16;
-  *bytes = static_cast<size_t>(opl::grid_limit()) * 2 * rows *
+  *bytes = static_cast<size_t>(opl::paged_grid_limit()) * 2 * rows *
            (sizeof(float) * static_cast<size_t>((head_dim + 1) / 2 * 2) + sizeof(float2));
   return cudaSuccess;
 }

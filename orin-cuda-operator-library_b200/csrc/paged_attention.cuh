@@ -127,15 +127,91 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedArgs& a, int unit) {
   return u;
 }
 
-// Grid and scratch of a launch: `ctas` CTAs, at most two partial units each.
-struct PagedPlan {
-  int rows;  // of a unit
-  int ctas;
-};
+__device__ __forceinline__ void st_out(float* p, float x) { *p = x; }
+__device__ __forceinline__ void st_out(__half* p, float x) { *p = __float2half_rn(x); }
+__device__ __forceinline__ void st_out(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-size_t paged_workspace_bytes(const PagedPlan& plan, int head_dim);
+// Joins the parts of the unit that CTA blockIdx.x of the main launch starts
+// and does not end (slot 1 of that CTA, slot 0 of the following ones), row
+// blockIdx.y, in key order.
+template <typename T, int kUnitTile, int kUnitLeast, int kRows>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int grid_ctas,
+                                                         int row_cap) {
+  __shared__ float top_of_warp[4];
+  pdl_begin();
+  int64_t at = 0, limit = 0;
+  const int cta = blockIdx.x;
+  const PagedStart start = paged_start<128, kUnitTile, kUnitLeast>(
+      a, grid_ctas, [&](long long total, int ctas) -> long long {
+        if (cta + 1 >= ctas) return -1;
+        limit = range_begin(total, ctas, cta + 1);
+        at = limit - 1;  // the last tile of the CTA
+        return at;
+      });
+  if (cta + 1 >= start.ctas) return;
+  const int sequence = start.sequence;
+  const int length = paged_length(a, sequence);
+  const int tiles = key_tiles(length, kUnitTile);
+  const Segment last = segment_at(at, limit, start.before, tiles, a.units());
+  if (last.end == tiles) return;  // not cut here
+  const int64_t unit_begin = at - last.begin;
+  if (unit_begin < range_begin(start.total, start.ctas, cta)) return;  // an earlier CTA starts it
+  const PagedUnit unit = paged_unit<kRows>(a, last.unit);
+  const int row = blockIdx.y;
+  if (row >= unit.rows) return;
+  const int end_cta = range_owner(start.total, start.ctas, unit_begin + tiles - 1);
+  const int parts = end_cta - cta + 1;
+  const auto part_row = [&](int p) {
+    const int slot = p == 0 ? 2 * cta + 1 : 2 * (cta + p);
+    return static_cast<int64_t>(slot) * row_cap + row;
+  };
+  float top = -INFINITY;
+  for (int p = threadIdx.x; p < parts; p += 128) top = fmaxf(top, __ldcg(&a.partial_ml[part_row(p)]).x);
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) top_of_warp[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(top_of_warp[0], top_of_warp[1]), fmaxf(top_of_warp[2], top_of_warp[3]));
+  const float base_m = top == -INFINITY ? 0.0f : top;
+  for (int d = threadIdx.x; d < a.head_dim; d += 128) {
+    float sum = 0.0f, out = 0.0f;
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+      const float2 ml = __ldcg(&a.partial_ml[part_row(p)]);
+      const float f = paged_exp2(ml.x - base_m);
+      sum = fmaf(f, ml.y, sum);
+      out = fmaf(f, __ldcg(&a.partial[part_row(p) * a.head_dim + d]), out);
+    }
+    st_out(static_cast<T*>(a.out) +
+               (static_cast<int64_t>(sequence) * a.heads + unit.first_head + row) * a.head_dim + d,
+           out / sum);
+  }
+}
 
-// The tensor-core kernel for 16-bit caches on 16-byte boundaries.
-bool paged_attention_mma_supported(const PagedArgs& a, size_t element);
+template <typename T, int kUnitTile, int kUnitLeast, int kRows>
+cudaError_t launch_join(const PagedArgs& a, int grid_ctas, int row_cap, cudaStream_t stream) {
+  return launch_pdl(paged_join_kernel<T, kUnitTile, kUnitLeast, kRows>,
+                    dim3(grid_ctas - 1, row_cap), dim3(128), stream, a, grid_ctas, row_cap);
+}
+
+// The most CTAs of a launch; the workspace is sized for them.
+inline int paged_grid_limit() { return 2 * sm_count(); }
+
+// CTAs of a launch: at most `limit`, and no more than the longest batch that
+// the block table can hold keeps busy.
+inline int paged_grid(const PagedArgs& a, int limit, int tile, int least, int unit_rows) {
+  const int64_t capacity = static_cast<int64_t>(a.max_pages) * a.page_size.divisor;
+  const int64_t tiles = capacity <= tile ? 1 : (capacity - 1) / tile + 1;
+  const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads *
+                        ((a.group + unit_rows - 1) / unit_rows);
+  // The product may pass 63 bits; then only its comparison with the limit counts.
+  const double total = static_cast<double>(tiles) * static_cast<double>(units);
+  if (total >= static_cast<double>(limit) * least) return limit;
+  return active_ctas(tiles * units, limit, least);
+}
+
+// The tensor-core kernel: 16-bit types, head_dim a multiple of 8, addresses
+// and strides multiples of 16 bytes.
+template <typename T>
+int paged_attention_mma(PagedArgs a, cudaStream_t stream);
 
 }  // namespace opl

@@ -431,6 +431,23 @@ def test_attention_infinities_and_nan_in_keys(ops, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("heads", [2, 12, 32])
+def test_attention_infinity_in_values(ops, dtype, heads):
+    """An infinite value leaves its column not finite in the heads that read
+    it, and nothing else changes."""
+    cache = Paged([40, 40], 2, 64, 16, dtype, 25)
+    q = randn(gen(1), 2, heads, 64, dtype=dtype)
+    clean = ops.paged_attention(q, cache.k, cache.v, cache.table, cache.seq_lens)
+    v = cache.v.clone()
+    v[cache.table[1, 0].long(), 5, 1, 9] = math.inf
+    got = ops.paged_attention(q, cache.k, v, cache.table, cache.seq_lens)
+    assert not torch.isfinite(got[1, heads // 2:, 9]).any()
+    same = torch.ones_like(got, dtype=torch.bool)
+    same[1, heads // 2:, 9] = False
+    assert torch.equal(got[same], clean[same])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
 def test_attention_bad_indices_are_reported(ops, dtype):
     """A page outside the cache is left out and reported; so is a length past
     the table's row, which is cut, and a negative one, which is empty."""
