@@ -9,21 +9,27 @@
 // to be written to shared memory in a swizzled layout (with V transposed), and
 // the rate is not what bounds.
 //
-// One warp owns 16 keys at a time and never waits for another one:
+// One warp owns 16 keys at a time and a ring of stages, a tile of keys and a
+// tile of values each; it never waits for another warp:
 //
-// * Every lane copies by cp.async exactly the 16-byte pieces that it will
-//   itself use as operands, into a ring of its own, kStages deep.  No barrier
-//   guards the ring, each piece is read back by a conflict-free 128-bit load,
-//   and 8 warps x 3 stages keep 192 KB (head size 128) in flight per SM; about
-//   50 KB cover the latency at the full rate.
-// * That works because a contraction may run over its index in any order.
-//   S = Q K^T: lane (g, t) of an m16n8k16 B operand holds row g (key g), any
-//   8 consecutive elements of the head per two instructions; Q is loaded in
-//   the same order.  O = P V: the operand pairs two keys of one column, so the
-//   lane loads 8 consecutive columns of keys 2t, 2t+1, 2t+8, 2t+9 -- the keys
-//   whose weights the S accumulator left in this lane -- and one byte permute
-//   a register pairs them; instruction e of 8 then computes columns 8n + e of
-//   the head, which lands 8 consecutive columns of a row in one lane.
+// * The tiles come by TMA (a box of 16 tokens x 64 columns of one head, 128-byte
+//   swizzle; two boxes of 8 tokens when 16 is no divisor of the page size).
+//   Copies by the lanes (cp.async), which every page size and stride allows,
+//   put the same layout there but take an instruction per 512 bytes and lane
+//   group: with 131071 keys, 32/8 heads of 128 in BF16, their issue alone
+//   bounds the kernel (106 us with no arithmetic, 138 us when a group of eight
+//   lanes does not cover 128 bytes of a row; TMA 97 us with it).  8 warps x 3
+//   stages keep 192 KB in flight per SM (5 x 5 or 6 x 4: 99-105 us).
+// * A contraction may run over its index in any order, so operands are read
+//   from that layout by conflict-free 128-bit loads, without ldmatrix.
+//   S = Q K^T: lane (g, t) of an m16n8k16 B operand holds row g (key g); two
+//   instructions take 8 consecutive elements of it, those at 16t + 8 (j & 1)
+//   of the 64-column box; Q is loaded in the same order.  O = P V: the operand
+//   pairs two keys of one column, so the lane loads 8 consecutive columns of
+//   keys 2t, 2t+1, 2t+8, 2t+9 -- the keys whose weights the S accumulator left
+//   in this lane -- and one byte permute a register pairs them; instruction e
+//   of 8 then computes columns 8n + e of the box, which lands 8 consecutive
+//   columns of a row in one lane.
 // * The weights enter P V as the sum of two 16-bit values, so that their
 //   rounding (2^-9 in BF16, as much as the result's own) does not show.  With
 //   up to 8 query heads a unit the second value rides in the 8 rows of the
@@ -31,13 +37,19 @@
 //
 // Running maximum, sum and output are FP32 in registers; the warps of a CTA
 // merge at the end of a segment, and cut units are joined by a second launch.
+#include <utility>
+
 #include "paged_attention.cuh"
+#include "tc_common.cuh"
+#include "tmap.cuh"
 
 namespace opl {
 
 namespace {
 
 constexpr int kTile = 16;
+// Block-table entries are loaded this many steps before their copies.
+constexpr int kAhead = 2;
 
 template <typename T>
 struct Mma;
@@ -112,33 +124,56 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
 // a unit.
 template <typename T, int kDim, int kRows, int kWarps, int kStages>
 struct Shape {
-  static constexpr int kKeyChunks = 2 * (kDim / 32);    // 16-byte pieces a lane and tile
-  static constexpr int kValueChunks = 4 * (kDim / 64);
-  static constexpr int kStageBytes = (kKeyChunks + kValueChunks) * 512;
+  static constexpr int kKeyBytes = kTile * kDim * 2;
+  static constexpr int kStageBytes = 2 * kKeyBytes;
   static constexpr int kRingBytes = kStages * kStageBytes;  // of a warp
   static constexpr int kPitch = kDim + 4;  // of a merged row, in floats
-  static constexpr size_t kShared = static_cast<size_t>(kWarps) * kRingBytes;
+  static constexpr size_t kShared = 1024 + static_cast<size_t>(kWarps) * kRingBytes;
   static_assert(kRows * kPitch * 4 <= kRingBytes, "a warp merges through its own ring");
-  static_assert(kShared <= 220 * 1024, "beside the static arrays");
+  static_assert(kShared <= 222 * 1024, "beside the static arrays");
 };
 
-template <typename T, int kDim, int kRows, int kWarps, int kStages, int kLeast>
-__global__ void __launch_bounds__(32 * kWarps, 1) paged_mma_kernel(const PagedArgs a, int row_cap) {
+// How the tensor maps of the caches are laid out.
+struct MapOrder {
+  int token_first;  // dimensions (head_dim, token, head, page), else head before token
+  int boxes;        // of a tile: one of 16 tokens, or two of 8
+};
+
+// Copies are made by the TMA unit, or by the lanes (kTma false).
+template <typename T, int kDim, int kRows, bool kTma, int kWarps, int kStages, int kLeast>
+__global__ void __launch_bounds__(32 * kWarps, 1)
+    paged_mma_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap k_map,
+                     const __grid_constant__ CUtensorMap v_map, const MapOrder order, int row_cap) {
   using S = Shape<T, kDim, kRows, kWarps, kStages>;
   constexpr int kThreads = 32 * kWarps;
   constexpr int kHalves = kRows / 8;  // row groups of the S accumulator in use
-  extern __shared__ __align__(16) unsigned char ring[];
+  extern __shared__ unsigned char shared[];
   __shared__ float merge_m[kWarps][kRows], merge_l[kWarps][kRows];
-  pdl_begin();
-
+  __shared__ uint64_t full[kWarps][kStages];
+  __shared__ int abort_wait;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const uint32_t my_ring =
-      static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + warp * S::kRingBytes + lane * 16;
+  unsigned char* const rings = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<std::uintptr_t>(shared) + 1023) & ~static_cast<std::uintptr_t>(1023));
+  unsigned char* const ring = rings + warp * S::kRingBytes;
+  if constexpr (kTma) {
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < kStages; ++i) tc::mbar_init(&full[warp][i], 1);
+      tc::fence_barrier_init();
+      if (warp == 0) {
+        abort_wait = 0;
+        tc::prefetch_tmap(&k_map);
+        tc::prefetch_tmap(&v_map);
+      }
+    }
+  }
+  pdl_begin();
+
   const T* q = static_cast<const T*>(a.q);
-  const T* keys = static_cast<const T*>(a.k);
-  const T* values = static_cast<const T*>(a.v);
   const int page_size = static_cast<int>(a.page_size.divisor);
+  // The barriers are also set up before the first copy by this search's
+  // __syncthreads.
   const PagedStart start = paged_start<kThreads, kTile, kLeast>(
       a, gridDim.x, [](long long total, int ctas) -> long long {
         return static_cast<int>(blockIdx.x) < ctas ? range_begin(total, ctas, blockIdx.x) : -1;
@@ -149,6 +184,14 @@ __global__ void __launch_bounds__(32 * kWarps, 1) paged_mma_kernel(const PagedAr
   int sequence = start.sequence;
   int64_t before = start.before;
   int reported = 0;
+  int slot_in = 0, slot_out = 0;  // ring stages being filled and read
+  uint32_t parity = 0;            // of the stage being read
+  bool dead = false;              // a wait gave up; the warp copies no more
+
+  // Where this lane's pieces lie in a stage (see the layout above).
+  const uint32_t k_piece = g * 128 + (2 * t ^ g) * 16;
+  const uint32_t v_piece = S::kKeyBytes + 2 * t * 128 + (g ^ 2 * t) * 16;
+  const uint32_t ring_address = tc::smem_u32(ring);
 
   while (w < limit) {
     const int raw_length = ld_int(a.seq_lens + sequence);
@@ -164,68 +207,85 @@ __global__ void __launch_bounds__(32 * kWarps, 1) paged_mma_kernel(const PagedAr
     w += segment.end - segment.begin;
     const PagedUnit unit = paged_unit<kRows>(a, segment.unit);
     const int* table = a.block_table + sequence * a.table_row;
-    const T* k_head = keys + unit.kv_head * a.k_head;
-    const T* v_head = values + unit.kv_head * a.v_head;
     const int first = segment.begin + warp;
-    const int count = first < segment.end ? (segment.end - first - 1) / kWarps + 1 : 0;
+    const int count = !dead && first < segment.end ? (segment.end - first - 1) / kWarps + 1 : 0;
 
-    // Lanes 0-15 place the keys of a tile, lanes 16-31 its values; the
-    // block-table entry is loaded a step before it is used.
+    // The key that this lane places in tile i: with the TMA unit the first of
+    // a box of 16 or 8 (even and odd lanes: first and second half of the
+    // tile), else lanes 0-15 a key each and lanes 16-31 their values.  Its
+    // block-table entry is loaded some steps before it is used.
+    const auto key_of = [&](int i) {
+      return (first + i * kWarps) * kTile + (kTma ? 8 * (lane & 1) : lane & 15);
+    };
     const auto fetch = [&](int i) {
-      const int key = (first + i * kWarps) * kTile + (lane & 15);
+      const int key = key_of(i);
       return i < count && key < length ? ld_int(table + fast_div(key, a.page_size)) : 0;
     };
-    // Copies tile i into its stage; bit j of the result: key j is there.
+    // Copies tile i into the next stage; bit j of the result: key j is there.
     const auto issue = [&](int i, int page) -> uint32_t {
       uint32_t there = 0;
       if (i < count) {
-        const int key = (first + i * kWarps) * kTile + (lane & 15);
-        int64_t place = -1;
-        if (key < length) {
-          if (cache_page(page, a.pages)) {
-            const int inside =
-                key - static_cast<int>(fast_div(key, a.page_size)) * page_size;
-            place = lane < 16 ? page * a.k_page + inside * a.k_token
-                              : page * a.v_page + inside * a.v_token;
-          } else {
-            reported = kBadPage;
+        const int key = key_of(i);
+        const bool known = key < length;
+        const bool ok = known && cache_page(page, a.pages);
+        if (known && !ok) reported = kBadPage;
+        const int inside = key - static_cast<int>(fast_div(key, a.page_size)) * page_size;
+        if constexpr (kTma) {
+          const uint32_t halves = __ballot_sync(kFullMask, ok) & 3u;
+          const int left = length - (first + i * kWarps) * kTile;
+          there = left >= kTile ? 0xffffu : (1u << left) - 1;
+          if ((halves & 1u) == 0) there &= 0xff00u;
+          if ((halves & 2u) == 0) there &= 0x00ffu;
+          uint64_t* const bar = &full[warp][slot_in];
+          if (lane == 0) tc::mbar_expect_tx(bar, S::kStageBytes);
+          __syncwarp();
+          if (lane < order.boxes) {
+            // A box that holds no key lies past the last page: zeros.
+            const int p = ok ? page : static_cast<int>(a.pages);
+            const int y = order.token_first ? inside : unit.kv_head;
+            const int z = order.token_first ? unit.kv_head : inside;
+            unsigned char* dst = ring + slot_in * S::kStageBytes + lane * 1024;
+#pragma unroll
+            for (int c = 0; c < kDim / 64; ++c)
+              tc::tma_load_4d(dst + c * 2048, &k_map, 64 * c, y, z, p, bar);
+#pragma unroll
+            for (int c = 0; c < kDim / 64; ++c)
+              tc::tma_load_4d(dst + S::kKeyBytes + c * 2048, &v_map, 64 * c, y, z, p, bar);
+          }
+        } else {
+          const int64_t place = !ok ? -1
+                                : lane < 16
+                                    ? page * a.k_page + inside * a.k_token + unit.kv_head * a.k_head
+                                    : page * a.v_page + inside * a.v_token + unit.kv_head * a.v_head;
+          there = __ballot_sync(kFullMask, ok) & 0xffffu;
+          // Eight lanes copy 128 bytes of one row.
+          const int piece = lane & 7;
+          uint32_t dst = ring_address + slot_in * S::kStageBytes;
+#pragma unroll
+          for (int s = 0; s < 8; ++s) {
+            const int row = 4 * (s & 3) + (lane >> 3);
+            const int64_t at = __shfl_sync(kFullMask, place, (s < 4 ? 0 : 16) + row);
+            const T* const src =
+                static_cast<const T*>(s < 4 ? a.k : a.v) + (at >= 0 ? at : 0) + 8 * piece;
+            const uint32_t to = dst + row * 128 + (piece ^ (row & 7)) * 16;
+#pragma unroll
+            for (int c = 0; c < kDim / 64; ++c)
+              copy16(to + (s < 4 ? 0 : S::kKeyBytes) + c * 2048, src + 64 * c,
+                     at >= 0 && 64 * c + 8 * piece < a.head_dim);
           }
         }
-        there = __ballot_sync(kFullMask, place >= 0) & 0xffffu;
-        uint32_t dst = my_ring + (i % kStages) * S::kStageBytes;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int64_t at = __shfl_sync(kFullMask, place, 8 * n + g);
-#pragma unroll
-          for (int j = 0; j < kDim / 32; ++j, dst += 512) {
-            const int d = 32 * j + 8 * t;
-            const bool ok = at >= 0 && d < a.head_dim;
-            copy16(dst, ok ? k_head + at + d : keys, ok);
-          }
-        }
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const int64_t at =
-              __shfl_sync(kFullMask, place, 16 + 2 * t + (i4 & 1) + 8 * (i4 >> 1));
-#pragma unroll
-          for (int c = 0; c < kDim / 64; ++c, dst += 512) {
-            const int d = 64 * c + 8 * g;
-            const bool ok = at >= 0 && d < a.head_dim;
-            copy16(dst, ok ? v_head + at + d : values, ok);
-          }
-        }
+        if (++slot_in == kStages) slot_in = 0;
       }
-      copy_commit();
+      if constexpr (!kTma) copy_commit();
       return there;
     };
 
     uint32_t there[kStages];
-    int pages[kStages];
+    int pages[kStages - 1 + kAhead];
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) pages[i] = fetch(i);
+    for (int i = 0; i < kStages - 1 + kAhead; ++i) pages[i] = fetch(i);
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) there[i] = issue(i, pages[i]);
-    int next_page = pages[kStages - 1];
 
     // Q in the order of the key pieces: words 0, 1 of piece j are the first
     // instruction's two k pairs, words 2, 3 the second's.
@@ -236,7 +296,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) paged_mma_kernel(const PagedAr
       const T* src = q + sequence * a.q_batch + (unit.first_head + row) * a.q_head;
 #pragma unroll
       for (int j = 0; j < kDim / 32; ++j) {
-        const int d = 32 * j + 8 * t;
+        const int d = 64 * (j / 2) + 16 * t + 8 * (j & 1);
         qa[j][h] = row < unit.rows && d < a.head_dim ? ld_ro(reinterpret_cast<const uint4*>(src + d))
                                                      : make_uint4(0, 0, 0, 0);
       }
@@ -251,18 +311,39 @@ __global__ void __launch_bounds__(32 * kWarps, 1) paged_mma_kernel(const PagedAr
     for (int h = 0; h < kHalves; ++h) m[h] = -INFINITY, l[h] = 0.0f;
 
     for (int i = 0; i < count; ++i) {
-      const int later_page = fetch(i + kStages);
-      there[kStages - 1] = issue(i + kStages - 1, next_page);
-      next_page = later_page;
-      copy_wait<kStages - 1>();
-      uint32_t src = my_ring + (i % kStages) * S::kStageBytes;
+      const int later_page = fetch(i + kStages - 1 + kAhead);
+      __syncwarp();  // every lane has read the stage that is filled next
+      there[kStages - 1] = issue(i + kStages - 1, pages[kStages - 1]);
+#pragma unroll
+      for (int x = kStages - 1; x < kStages - 2 + kAhead; ++x) pages[x] = pages[x + 1];
+      pages[kStages - 2 + kAhead] = later_page;
+      if constexpr (kTma) {
+        if (!tc::mbar_wait_warp(&full[warp][slot_out], parity, &abort_wait, a.watchdog,
+                                tc::kWatchdogPaged)) {
+          // Give the other copies in flight the same time to land, then leave
+          // the segment; the output is not valid and the watchdog says so.
+          for (int x = 1; x < kStages && i + x < count; ++x) {
+            const int slot = (slot_out + x) % kStages;
+            volatile int alone = 0;
+            tc::mbar_wait(&full[warp][slot], slot < slot_out ? parity ^ 1u : parity, &alone,
+                          a.watchdog, tc::kWatchdogPaged);
+          }
+          dead = true;
+          break;
+        }
+      } else {
+        copy_wait<kStages - 1>();
+        __syncwarp();  // what the other lanes copied
+      }
+      const uint32_t stage = ring_address + slot_out * S::kStageBytes;
+      if (++slot_out == kStages) slot_out = 0, parity ^= 1u;
 
       float s[2][4] = {};
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int j = 0; j < kDim / 32; ++j, src += 512) {
-          const uint4 b = ld_shared(src);
+        for (int j = 0; j < kDim / 32; ++j) {
+          const uint4 b = ld_shared(stage + (k_piece ^ (j & 1) * 16) + (j / 2) * 2048 + n * 1024);
           Mma<T>::run(s[n], qa[j][0].x, kHalves == 2 ? qa[j][kHalves - 1].x : 0u, qa[j][0].y,
                       kHalves == 2 ? qa[j][kHalves - 1].y : 0u, b.x, b.y);
           Mma<T>::run(s[n], qa[j][0].z, kHalves == 2 ? qa[j][kHalves - 1].z : 0u, qa[j][0].w,
@@ -272,12 +353,13 @@ __global__ void __launch_bounds__(32 * kWarps, 1) paged_mma_kernel(const PagedAr
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int x = 0; x < 2 * kHalves; ++x) s[n][x] *= a.scale_log2;
-      if (there[0] != 0xffffu) {
+      const uint32_t seen = there[0];
+      if (seen != 0xffffu) {
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int x = 0; x < 2 * kHalves; ++x)
-            if ((there[0] >> (8 * n + 2 * t + (x & 1)) & 1u) == 0) s[n][x] = -INFINITY;
+            if ((seen >> (8 * n + 2 * t + (x & 1)) & 1u) == 0) s[n][x] = -INFINITY;
       }
 #pragma unroll
       for (int x = 0; x + 1 < kStages; ++x) there[x] = there[x + 1];
@@ -323,7 +405,14 @@ __global__ void __launch_bounds__(32 * kWarps, 1) paged_mma_kernel(const PagedAr
       for (int c = 0; c < kDim / 64; ++c) {
         uint4 v[4];
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) v[i4] = ld_shared(src + (i4 * (kDim / 64) + c) * 512);
+        for (int x = 0; x < 4; ++x)  // keys 2t, 2t + 1, 2t + 8, 2t + 9
+          v[x] = ld_shared(stage + (x & 1 ? (v_piece ^ 16) + 128 : v_piece) + c * 2048 +
+                           (x >> 1) * 1024);
+        if (seen != 0xffffu) {  // what lies behind the length is not a value
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if ((seen >> (2 * t + (x & 1) + 8 * (x >> 1)) & 1u) == 0) v[x] = make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           uint32_t b0, b1;
@@ -345,7 +434,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) paged_mma_kernel(const PagedAr
         }
       }
     }
-    copy_wait<0>();
+    if constexpr (!kTma) copy_wait<0>();
 
     // Merge the warps, each through its own (now empty) ring.
 #pragma unroll
@@ -358,7 +447,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) paged_mma_kernel(const PagedAr
       }
     }
     __syncwarp();  // the ring is written across lanes from here
-    float* const merge_o = reinterpret_cast<float*>(ring + warp * S::kRingBytes);
+    float* const merge_o = reinterpret_cast<float*>(ring);
 #pragma unroll
     for (int h = 0; h < kHalves; ++h)
 #pragma unroll
@@ -396,7 +485,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) paged_mma_kernel(const PagedAr
       for (int x = 0; x < kWarps; ++x) {
         const float f = paged_exp2(merge_m[x][r] - base_m);
         sum = fmaf(f, merge_l[x][r], sum);
-        out = fmaf(f, reinterpret_cast<const float*>(ring + x * S::kRingBytes)[r * S::kPitch + d],
+        out = fmaf(f, reinterpret_cast<const float*>(rings + x * S::kRingBytes)[r * S::kPitch + d],
                    out);
       }
       if (segment.whole()) {
@@ -409,15 +498,45 @@ __global__ void __launch_bounds__(32 * kWarps, 1) paged_mma_kernel(const PagedAr
         if (d == 0) a.partial_ml[row] = make_float2(top, sum);
       }
     }
+    // The rings go back to the TMA unit.
+    if constexpr (kTma) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
   }
   if (reported != 0) watchdog_trip(a.watchdog, reported);
 }
 
-template <typename T, int kDim, int kRows, int kWarps, int kStages>
-int launch_mma(PagedArgs a, cudaStream_t stream) {
+// Encodes a cache for the TMA unit; false when its layout does not allow it.
+template <typename T>
+bool cache_map(CUtensorMap* map, const PagedArgs& a, const void* base, int64_t page, int64_t token,
+               int64_t head, const MapOrder& order) {
+  const uint64_t page_size = a.page_size.divisor;
+  uint64_t extent[4] = {static_cast<uint64_t>(a.head_dim), page_size,
+                        static_cast<uint64_t>(a.kv_heads), static_cast<uint64_t>(a.pages)};
+  int64_t stride[3] = {token, head, page};
+  uint32_t box[4] = {64, static_cast<uint32_t>(kTile / order.boxes), 1, 1};
+  if (!order.token_first) {
+    std::swap(extent[1], extent[2]);
+    std::swap(stride[0], stride[1]);
+    std::swap(box[1], box[2]);
+  }
+  uint64_t bytes[3];
+  for (int i = 0; i < 3; ++i) {
+    // A dimension of one element may come with any stride.
+    if (extent[i + 1] == 1) stride[i] = 8;
+    if (stride[i] <= 0 || stride[i] >= (int64_t{1} << 39)) return false;
+    bytes[i] = static_cast<uint64_t>(stride[i]) * sizeof(T);
+  }
+  const CUtensorMapDataType type = sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  return encode_tmap(map, type, 4, base, extent, bytes, box, CU_TENSOR_MAP_SWIZZLE_128B) ==
+         cudaSuccess;
+}
+
+template <typename T, int kDim, int kRows, bool kTma, int kWarps, int kStages>
+int launch_mma(PagedArgs a, const CUtensorMap& k_map, const CUtensorMap& v_map,
+               const MapOrder& order, cudaStream_t stream) {
   constexpr int kLeast = kWarps;
-  constexpr auto kernel = paged_mma_kernel<T, kDim, kRows, kWarps, kStages, kLeast>;
+  constexpr auto kernel = paged_mma_kernel<T, kDim, kRows, kTma, kWarps, kStages, kLeast>;
   constexpr size_t kShared = Shape<T, kDim, kRows, kWarps, kStages>::kShared;
   a.parts = (a.group + kRows - 1) / kRows;
   const int row_cap = a.group < kRows ? a.group : kRows;
@@ -437,26 +556,40 @@ int launch_mma(PagedArgs a, cudaStream_t stream) {
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
-  error = cudaLaunchKernelEx(&config, kernel, a, row_cap);
+  error = cudaLaunchKernelEx(&config, kernel, a, k_map, v_map, order, row_cap);
   if (error == cudaSuccess && grid > 1)
     error = launch_join<T, kTile, kLeast, kRows>(a, grid, row_cap, stream);
   return error != cudaSuccess ? error : cudaGetLastError();
 }
 
-template <typename T, int kRows>
-int pick_dim(const PagedArgs& a, cudaStream_t stream) {
+template <typename T, int kRows, bool kTma>
+int pick_dim(const PagedArgs& a, const CUtensorMap& k_map, const CUtensorMap& v_map,
+             const MapOrder& order, cudaStream_t stream) {
   // About 192 KB of rings a CTA, one CTA a SM.
-  if (a.head_dim <= 64) return launch_mma<T, 64, kRows, 8, 6>(a, stream);
-  if (a.head_dim <= 128) return launch_mma<T, 128, kRows, 8, 3>(a, stream);
-  if (a.head_dim <= 192) return launch_mma<T, 192, kRows, 4, 4>(a, stream);
-  return launch_mma<T, 256, kRows, 4, 3>(a, stream);
+  if (a.head_dim <= 64) return launch_mma<T, 64, kRows, kTma, 8, 6>(a, k_map, v_map, order, stream);
+  if (a.head_dim <= 128)
+    return launch_mma<T, 128, kRows, kTma, 8, 3>(a, k_map, v_map, order, stream);
+  if (a.head_dim <= 192)
+    return launch_mma<T, 192, kRows, kTma, 4, 4>(a, k_map, v_map, order, stream);
+  return launch_mma<T, 256, kRows, kTma, 4, 3>(a, k_map, v_map, order, stream);
 }
 
 }  // namespace
 
 template <typename T>
 int paged_attention_mma(PagedArgs a, cudaStream_t stream) {
-  return a.group <= 8 ? pick_dim<T, 8>(a, stream) : pick_dim<T, 16>(a, stream);
+  if (a.pages > 0x7fffffff) a.pages = 0x7fffffff;  // as far as block-table entries reach
+  CUtensorMap k_map = {}, v_map = {};
+  MapOrder order = {a.k_token < a.k_head ? 1 : 0, a.page_size.divisor % kTile == 0 ? 1 : 2};
+  const bool tma =
+      a.page_size.divisor % 8 == 0 &&
+      cache_map<T>(&k_map, a, a.k, a.k_page, a.k_token, a.k_head, order) &&
+      cache_map<T>(&v_map, a, a.v, a.v_page, a.v_token, a.v_head, order);
+  if (tma)
+    return a.group <= 8 ? pick_dim<T, 8, true>(a, k_map, v_map, order, stream)
+                        : pick_dim<T, 16, true>(a, k_map, v_map, order, stream);
+  return a.group <= 8 ? pick_dim<T, 8, false>(a, k_map, v_map, order, stream)
+                      : pick_dim<T, 16, false>(a, k_map, v_map, order, stream);
 }
 
 template int paged_attention_mma<__half>(PagedArgs, cudaStream_t);

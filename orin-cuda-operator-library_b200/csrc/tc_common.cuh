@@ -14,6 +14,7 @@ namespace tc {
 // Watchdog codes written when a bounded wait gives up.
 constexpr int kWatchdogGemm = 0x6e01;
 constexpr int kWatchdogAttention = 0x6e02;
+constexpr int kWatchdogPaged = 0x6e05;
 // A wait is declared hung after kMaxWaitNs of wall time (read from
 // %globaltimer every 256 polls), or after kMaxPolls polls of
 // mbarrier.try_wait as a backstop.  Both are far beyond any legitimate wait
@@ -111,6 +112,16 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// 4-D tiled load.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y,
+                                            int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
 
