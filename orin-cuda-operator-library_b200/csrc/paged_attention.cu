@@ -14,8 +14,7 @@
 // A warp takes 8 keys at a time: E products a lane, row and key; the 8 x rows
 // sums over 32 lanes by a transposing butterfly (about one shuffle a sum
 // instead of five); one exponential a key and row; running maximum and sum
-// (log2 domain) and the output in registers.  The warps of a CTA take the
-// tiles of a segment in turn and merge through shared memory at its end.
+// (log2 domain) and the output in registers.
 #include "paged_attention.cuh"
 
 namespace opl {
@@ -25,7 +24,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTile = 8;  // keys of a warp's step
-constexpr int kLeast = kWarps;
 
 template <typename T>
 __device__ __forceinline__ float ld_f32(const T* p);
@@ -114,14 +112,15 @@ __device__ __forceinline__ void transpose_sum(float (&v)[kCount], int lane) {
 constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
 
 template <typename T, int kRows, int E, bool kVec>
-__global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a, int row_cap) {
+__global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a) {
   constexpr int kSums = kTile * kRows;  // value index: row * kTile + key
   constexpr int kHeld = kSums > 32 ? kSums / 32 : 1;
   constexpr int kWidth = 32 * E;
   __shared__ float weights[kWarps][kRows][kTile];
   __shared__ float rescale[kWarps][kRows];
-  __shared__ float merge_m[kWarps][kRows], merge_l[kWarps][kRows];
-  extern __shared__ float merge_o[];  // [kWarps][kRows][kWidth]
+  __shared__ PagedParts<kWarps, kRows> parts;
+  __shared__ PagedStart starts[kWarps];
+  extern __shared__ __align__(16) float rows[];  // [kWarps][kRows][kWidth]
   pdl_begin();
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -129,15 +128,20 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a,
   const T* keys = static_cast<const T*>(a.k);
   const T* values = static_cast<const T*>(a.v);
   const int page_size = static_cast<int>(a.page_size.divisor);
-  const PagedStart start = paged_start<kThreads, kTile, kLeast>(
-      a, gridDim.x, [](long long total, int ctas) -> long long {
-        return static_cast<int>(blockIdx.x) < ctas ? range_begin(total, ctas, blockIdx.x) : -1;
+  if (lane < 2) parts.records[warp][lane] = PartRecord{};
+  const PagedTotal total = paged_start<kThreads, kTile, kWarps>(
+      a, gridDim.x, starts, [](const PagedTotal& x, int target) -> long long {
+        return static_cast<int>(blockIdx.x) < x.ctas
+                   ? x.ranges.begin(int64_t{kWarps} * blockIdx.x + target)
+                   : -1;
       });
-  if (static_cast<int>(blockIdx.x) >= start.ctas) return;
-  int64_t w = range_begin(start.total, start.ctas, blockIdx.x);
-  const int64_t limit = range_begin(start.total, start.ctas, blockIdx.x + 1);
-  int sequence = start.sequence;
-  int64_t before = start.before;
+  if (static_cast<int>(blockIdx.x) >= total.ctas) return;
+  const int64_t range = int64_t{kWarps} * blockIdx.x + warp;
+  int64_t w = total.ranges.begin(range);
+  const int64_t limit = total.ranges.begin(range + 1);
+  const bool opens = w == total.ranges.begin(int64_t{kWarps} * blockIdx.x);
+  int sequence = starts[warp].sequence;
+  int64_t before = starts[warp].before;
   int reported = 0;
 
   // Which row's score this lane holds after transpose_sum: the value index is
@@ -151,14 +155,15 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a,
     const int length = readable_length(raw_length, a.max_pages, page_size);
     if (length != raw_length) reported = kBadLength;
     const int tiles = key_tiles(length, kTile);
-    if (w >= (before + tiles) * a.units()) {
+    if (w >= (before + tiles) * a.units.divisor) {
       before += tiles;
       ++sequence;
       continue;
     }
-    const Segment segment = segment_at(w, limit, before, tiles, a.units());
-    w += segment.end - segment.begin;
-    const PagedUnit unit = paged_unit<kRows>(a, segment.unit);
+    const TilePlace at = place_of(w, before, tiles, a.units.divisor);
+    const int end = tiles - at.tile <= limit - w ? tiles : static_cast<int>(at.tile + (limit - w));
+    w += end - at.tile;
+    const PagedUnit unit = paged_unit<kRows>(a, at.unit);
     const int* table = a.block_table + sequence * a.table_row;
     const T* k_head = keys + unit.kv_head * a.k_head;
     const T* v_head = values + unit.kv_head * a.v_head;
@@ -175,7 +180,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a,
     }
     float m = -INFINITY, l = 0.0f;  // of my_row; l over my keys only
 
-    for (int tile = segment.begin + warp; tile < segment.end; tile += kWarps) {
+    for (int tile = at.tile; tile < end; ++tile) {
       const int base = tile * kTile;
       // Lanes 0-7 place the tile's keys, lanes 8-15 its values.
       int64_t place = -1;
@@ -255,60 +260,59 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a,
       }
     }
 
-    // Merge the warps: every lane that holds a row has its maximum; the sum
-    // is over the lanes (and, where several lanes hold the same key, one of
-    // them).
-    float l_row = l;
+    // Every lane that holds a row has its maximum; the sum is over the lanes
+    // that hold different keys of it.
     constexpr int kRowLanes = kRows >= 4 ? 32 / kRows : 8;
     constexpr int kFirst = kRows >= 4 ? 1 : 4 / kRows;
 #pragma unroll
-    for (int x = 1; x < kRowLanes; x <<= 1)
-      l_row += __shfl_xor_sync(kFullMask, l_row, x * kFirst);
-    if (my_key == 0) {
-      merge_m[warp][my_row] = m;
-      merge_l[warp][my_row] = l_row;
+    for (int x = 1; x < kRowLanes; x <<= 1) l += __shfl_xor_sync(kFullMask, l, x * kFirst);
+    constexpr int kLanesOfRow = 32 / kRows;  // lane of row r: the first of these
+    if (at.tile == 0 && end == tiles) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const float sum = __shfl_sync(kFullMask, l, r * kLanesOfRow);
+        if (r >= unit.rows) continue;
+        T* const dst = static_cast<T*>(a.out) +
+                       (static_cast<int64_t>(sequence) * a.heads + unit.first_head + r) * a.head_dim;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int d = column<E, kVec>(lane, e);
+          if (d < a.head_dim) st_out(dst + d, length == 0 ? 0.0f : o[r][e] / sum);
+        }
+      }
+      continue;
+    }
+    // A part: to shared memory when the warp is done, else out of its way.
+    const int kind = at.tile == 0 ? kTail : kHead;
+    const bool spilled = w < limit;
+    float* const part =
+        spilled ? a.spill + range * a.row_cap * a.head_dim : rows + warp * kRows * kWidth;
+    const int pitch = spilled ? a.head_dim : kWidth;
+    if (lane % kLanesOfRow == 0 && my_row < unit.rows) {
+      parts.m[warp][kind][my_row] = m;
+      parts.l[warp][kind][my_row] = l;
     }
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
+    for (int r = 0; r < kRows; ++r) {
+      if (r >= unit.rows) continue;
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        merge_o[(warp * kRows + r) * kWidth + column<E, kVec>(lane, e)] = o[r][e];
-    __syncthreads();
-    const int slot = 2 * blockIdx.x + segment.slot();
-    for (int i = threadIdx.x; i < unit.rows * a.head_dim; i += kThreads) {
-      const int r = i / a.head_dim, d = i - r * a.head_dim;
-      float top = -INFINITY;
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) top = fmaxf(top, merge_m[x][r]);
-      const float base_m = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f, out = 0.0f;
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) {
-        const float f = paged_exp2(merge_m[x][r] - base_m);
-        sum = fmaf(f, merge_l[x][r], sum);
-        out = fmaf(f, merge_o[(x * kRows + r) * kWidth + d], out);
-      }
-      if (segment.whole()) {
-        st_out(static_cast<T*>(a.out) +
-                   (static_cast<int64_t>(sequence) * a.heads + unit.first_head + r) * a.head_dim + d,
-               length == 0 ? 0.0f : out / sum);
-      } else {
-        const int64_t row = static_cast<int64_t>(slot) * row_cap + r;
-        a.partial[row * a.head_dim + d] = out;
-        if (d == 0) a.partial_ml[row] = make_float2(top, sum);
+      for (int e = 0; e < E; ++e) {
+        const int d = column<E, kVec>(lane, e);
+        if (d < a.head_dim) part[r * pitch + d] = o[r][e];
       }
     }
-    __syncthreads();
+    if (lane == 0)
+      parts.records[warp][kind] = PartRecord{sequence, at.unit, tiles,  at.tile,
+                                             end,      opens && kind == kHead, spilled};
   }
   if (reported != 0) watchdog_trip(a.watchdog, reported);
+  __syncthreads();
+  paged_merge<T, kWarps, kRows, kRows * kWidth, kWidth, kVec ? 4 : 1>(a, parts, rows);
 }
 
 template <typename T, int kRows, int E, bool kVec>
 int launch_simt(PagedArgs a, int grid_ctas, cudaStream_t stream) {
-  a.parts = (a.group + kRows - 1) / kRows;
-  const int row_cap = a.group < kRows ? a.group : kRows;
-  a.partial_ml = reinterpret_cast<float2*>(a.partial + static_cast<int64_t>(grid_ctas) * 2 *
-                                                           row_cap * a.head_dim);
+  paged_scratch(&a, grid_ctas, kWarps, kRows);
   constexpr size_t kShared = sizeof(float) * kWarps * kRows * 32 * E;
   static_assert(kShared <= 40 * 1024, "fits without an opt-in");
   cudaLaunchConfig_t config = {};
@@ -321,9 +325,9 @@ int launch_simt(PagedArgs a, int grid_ctas, cudaStream_t stream) {
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
-  cudaError_t error = cudaLaunchKernelEx(&config, paged_simt_kernel<T, kRows, E, kVec>, a, row_cap);
+  cudaError_t error = cudaLaunchKernelEx(&config, paged_simt_kernel<T, kRows, E, kVec>, a);
   if (error == cudaSuccess && grid_ctas > 1)
-    error = launch_join<T, kTile, kLeast, kRows>(a, grid_ctas, row_cap, stream);
+    error = launch_join<T, kTile, kWarps, kRows>(a, grid_ctas, stream);
   return error != cudaSuccess ? error : cudaGetLastError();
 }
 
@@ -342,7 +346,7 @@ bool aligned_rows(const PagedArgs& a, size_t element, int vector) {
                              a.v_page,  a.v_token, a.v_head, a.head_dim};
   for (int64_t s : strides)
     if (s % vector != 0) return false;
-  for (const void* p : {a.q, a.k, a.v})
+  for (const void* p : {a.q, a.k, a.v, static_cast<const void*>(a.out)})
     if (reinterpret_cast<std::uintptr_t>(p) % bytes != 0) return false;
   return true;
 }
@@ -395,7 +399,7 @@ int paged_attention(const void* q, int64_t q_batch, int64_t q_head, const opl_kv
   if constexpr (sizeof(T) == 2) {
     if (aligned_rows(a, sizeof(T), 8)) return paged_attention_mma<T>(a, stream);
   }
-  const int grid = paged_grid(a, paged_grid_limit(), kTile, kLeast, a.group <= 4 ? a.group : 4);
+  const int grid = paged_grid(a, paged_grid_limit(), kTile, kWarps, a.group <= 4 ? a.group : 4);
   if constexpr (sizeof(T) == 4) {
     if (vec && a.head_dim <= 64) return pick_rows<T, 2, true>(a, grid, stream);
     if (vec && a.head_dim <= 128) return pick_rows<T, 4, true>(a, grid, stream);
@@ -415,10 +419,7 @@ int opl_paged_attention_workspace(int heads, int kv_heads, int head_dim, size_t*
   if (bytes == nullptr || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 ||
       head_dim > opl::kPagedMaxHeadDim)
     return cudaErrorInvalidValue;
-  // Two partial units a CTA, up to 16 rows each, and their maxima and sums.
-  const size_t rows = heads / kv_heads < 16 ? heads / kv_heads : 16;
-  *bytes = static_cast<size_t>(opl::paged_grid_limit()) * 2 * rows *
-           (sizeof(float) * static_cast<size_t>((head_dim + 1) / 2 * 2) + sizeof(float2));
+  *bytes = opl::paged_scratch_bytes(heads / kv_heads, head_dim);
   return cudaSuccess;
 }
 

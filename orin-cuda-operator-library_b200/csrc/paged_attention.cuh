@@ -25,13 +25,14 @@ struct PagedArgs {
   FastDiv page_size;
   int max_pages, batch, heads, kv_heads, head_dim;
   int group;          // query heads of a key-value head
-  int parts;          // units a key-value head's query heads are cut into
+  FastDiv parts;      // units a key-value head's query heads are cut into
+  FastDiv units;      // of a sequence: key-value heads times parts
   float scale_log2;   // score scale times log2(e)
-  float* partial;     // [ctas][2][rows][head_dim], not normalised
-  float2* partial_ml; // [ctas][2][rows]: maximum (log2 domain) and sum
+  int row_cap;         // the most rows of a unit, min(group, the kernel's)
+  float* partial;      // [ctas][2][row_cap][head_dim], not normalised
+  float2* partial_ml;  // [ctas][2][row_cap]: maximum (log2 domain) and sum
+  float* spill;        // [ctas * warps][row_cap][head_dim]: heads of warps
   int* watchdog;
-
-  __device__ __forceinline__ int units() const { return kv_heads * parts; }
 };
 
 // 2^x on the MUFU ex2 unit (relative error about 2^-22).
@@ -53,21 +54,28 @@ __device__ __forceinline__ int paged_length(const PagedArgs& a, int sequence) {
                          static_cast<int>(a.page_size.divisor));
 }
 
+// Where a search for a tile ended.
 struct PagedStart {
-  int64_t total;   // tiles of all units
-  int64_t before;  // see segment_at
+  int64_t before;  // see place_of
   int sequence;
-  int ctas;  // that take part
+};
+
+struct PagedTotal {
+  int64_t tiles;  // of all units
+  int ctas;       // that take part
+  Ranges ranges;  // of their warps
 };
 
 // The whole CTA (kThreads threads) adds up the sequences' tiles and finds the
-// sequence of the tile that `place(total, ctas)` names.
-template <int kThreads, int kTile, int kLeast, typename Place>
-__device__ __forceinline__ PagedStart paged_start(const PagedArgs& a, int grid_ctas, Place place) {
+// sequences of kTargets tiles: target x is the tile place(total, x), or none
+// when that is negative.  kUnitWarps: warps of a CTA of the main launch.
+template <int kThreads, int kTile, int kUnitWarps, int kTargets, typename Place>
+__device__ __forceinline__ PagedTotal paged_start(const PagedArgs& a, int grid_ctas,
+                                                  PagedStart (&found)[kTargets], Place place) {
   constexpr int kWarpCount = kThreads / 32;
+  static_assert(kTargets <= kThreads, "a thread for each target");
   __shared__ long long warp_total[kWarpCount];
-  __shared__ long long found_before;
-  __shared__ int found;
+  __shared__ long long wanted[kTargets];
   const int tid = threadIdx.x;
   const int per = (a.batch + kThreads - 1) / kThreads;
   const int first = min(tid * per, a.batch), last = min(first + per, a.batch);
@@ -81,35 +89,45 @@ __device__ __forceinline__ PagedStart paged_start(const PagedArgs& a, int grid_c
   }
   if ((tid & 31) == 31) warp_total[tid >> 5] = running;
   __syncthreads();
-  long long before = running - mine, total = 0;
+  long long before = running - mine, all = 0;
 #pragma unroll
   for (int w = 0; w < kWarpCount; ++w) {
     if (w < (tid >> 5)) before += warp_total[w];
-    total += warp_total[w];
+    all += warp_total[w];
   }
-  PagedStart s;
-  s.total = total * a.units();
-  s.ctas = active_ctas(s.total, grid_ctas, kLeast);
-  const long long at = place(s.total, s.ctas);
-  if (at >= 0 && at < s.total) {
-    const long long wanted = at / a.units();
-    if (wanted >= before && wanted < before + mine) {
-      long long p = before;
-      for (int b = first; b < last; ++b) {
-        const int tiles = key_tiles(paged_length(a, b), kTile);
-        if (wanted < p + tiles) {
-          found = b;
-          found_before = p;
-          break;
-        }
-        p += tiles;
+  PagedTotal total;
+  total.tiles = all * a.units.divisor;
+  total.ctas = active_ctas(total.tiles, grid_ctas, kUnitWarps);  // a tile for each warp
+  total.ranges = make_ranges(total.tiles, kUnitWarps * total.ctas);
+  if (tid < kTargets) {
+    const long long at = place(total, tid);
+    wanted[tid] = at < 0 || at >= total.tiles ? -1
+                  : at >> 31 == 0             ? fast_div(static_cast<uint32_t>(at), a.units)
+                                              : at / a.units.divisor;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < kTargets; ++x) {
+    const long long to = wanted[x];
+    if (to < before || to >= before + mine) continue;
+    if (per == 1) {
+      found[x].sequence = tid;
+      found[x].before = before;
+      continue;
+    }
+    long long p = before;
+    for (int b = first; b < last; ++b) {
+      const int tiles = key_tiles(paged_length(a, b), kTile);
+      if (to < p + tiles) {
+        found[x].sequence = b;
+        found[x].before = p;
+        break;
       }
+      p += tiles;
     }
   }
   __syncthreads();
-  s.sequence = found;
-  s.before = found_before;
-  return s;
+  return total;
 }
 
 // Rows of one unit and where its queries lie.
@@ -120,8 +138,8 @@ struct PagedUnit {
 template <int kRows>
 __device__ __forceinline__ PagedUnit paged_unit(const PagedArgs& a, int unit) {
   PagedUnit u;
-  u.kv_head = unit / a.parts;
-  const int part = unit - u.kv_head * a.parts;
+  u.kv_head = static_cast<int>(fast_div(unit, a.parts));
+  const int part = unit - u.kv_head * static_cast<int>(a.parts.divisor);
   u.first_head = u.kv_head * a.group + part * kRows;
   u.rows = min(kRows, a.group - part * kRows);
   return u;
@@ -131,66 +149,207 @@ __device__ __forceinline__ void st_out(float* p, float x) { *p = x; }
 __device__ __forceinline__ void st_out(__half* p, float x) { *p = __float2half_rn(x); }
 __device__ __forceinline__ void st_out(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// Joins the parts of the unit that CTA blockIdx.x of the main launch starts
-// and does not end (slot 1 of that CTA, slot 0 of the following ones), row
-// blockIdx.y, in key order.
-template <typename T, int kUnitTile, int kUnitLeast, int kRows>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int grid_ctas,
-                                                         int row_cap) {
-  __shared__ float top_of_warp[4];
-  pdl_begin();
-  int64_t at = 0, limit = 0;
-  const int cta = blockIdx.x;
-  const PagedStart start = paged_start<128, kUnitTile, kUnitLeast>(
-      a, grid_ctas, [&](long long total, int ctas) -> long long {
-        if (cta + 1 >= ctas) return -1;
-        limit = range_begin(total, ctas, cta + 1);
-        at = limit - 1;  // the last tile of the CTA
-        return at;
-      });
-  if (cta + 1 >= start.ctas) return;
-  const int sequence = start.sequence;
-  const int length = paged_length(a, sequence);
-  const int tiles = key_tiles(length, kUnitTile);
-  const Segment last = segment_at(at, limit, start.before, tiles, a.units());
-  if (last.end == tiles) return;  // not cut here
-  const int64_t unit_begin = at - last.begin;
-  if (unit_begin < range_begin(start.total, start.ctas, cta)) return;  // an earlier CTA starts it
-  const PagedUnit unit = paged_unit<kRows>(a, last.unit);
-  const int row = blockIdx.y;
-  if (row >= unit.rows) return;
-  const int end_cta = range_owner(start.total, start.ctas, unit_begin + tiles - 1);
-  const int parts = end_cta - cta + 1;
-  const auto part_row = [&](int p) {
-    const int slot = p == 0 ? 2 * cta + 1 : 2 * (cta + p);
-    return static_cast<int64_t>(slot) * row_cap + row;
-  };
-  float top = -INFINITY;
-  for (int p = threadIdx.x; p < parts; p += 128) top = fmaxf(top, __ldcg(&a.partial_ml[part_row(p)]).x);
-  top = warp_max(top);
-  if ((threadIdx.x & 31) == 0) top_of_warp[threadIdx.x >> 5] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(top_of_warp[0], top_of_warp[1]), fmaxf(top_of_warp[2], top_of_warp[3]));
-  const float base_m = top == -INFINITY ? 0.0f : top;
-  for (int d = threadIdx.x; d < a.head_dim; d += 128) {
-    float sum = 0.0f, out = 0.0f;
-#pragma unroll 4
-    for (int p = 0; p < parts; ++p) {
-      const float2 ml = __ldcg(&a.partial_ml[part_row(p)]);
-      const float f = paged_exp2(ml.x - base_m);
-      sum = fmaf(f, ml.y, sum);
-      out = fmaf(f, __ldcg(&a.partial[part_row(p) * a.head_dim + d]), out);
-    }
-    st_out(static_cast<T*>(a.out) +
-               (static_cast<int64_t>(sequence) * a.heads + unit.first_head + row) * a.head_dim + d,
-           out / sum);
+// Stores kWidth consecutive elements.
+template <int kWidth, typename T>
+__device__ __forceinline__ void st_row(T* p, const float (&x)[kWidth]) {
+  if constexpr (kWidth == 1) {
+    st_out(p, x[0]);
+  } else {
+    static_assert(kWidth == 4, "one or four");
+    alignas(4 * sizeof(T)) T y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) st_out(&y[i], x[i]);
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(y);
+    else
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(y);
   }
 }
 
-template <typename T, int kUnitTile, int kUnitLeast, int kRows>
-cudaError_t launch_join(const PagedArgs& a, int grid_ctas, int row_cap, cudaStream_t stream) {
-  return launch_pdl(paged_join_kernel<T, kUnitTile, kUnitLeast, kRows>,
-                    dim3(grid_ctas - 1, row_cap), dim3(128), stream, a, grid_ctas, row_cap);
+template <int kWidth>
+__device__ __forceinline__ void ld_row(const float* p, bool global, float (&x)[kWidth]) {
+  if constexpr (kWidth == 4) {
+    const float4 v = global ? __ldcg(reinterpret_cast<const float4*>(p))
+                            : *reinterpret_cast<const float4*>(p);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    x[0] = global ? __ldcg(p) : *p;
+  }
+}
+
+// What the warps of a CTA leave for one another in shared memory.
+template <int kWarps, int kRows>
+struct PagedParts {
+  PartRecord records[kWarps][2];
+  float m[kWarps][2][kRows], l[kWarps][2][kRows];  // log2 domain; sums
+};
+
+// Joins the parts that the CTA's warps left, after a __syncthreads, and writes
+// each unit to the output or, when it reaches past the CTA, to the CTA's
+// partial slots.  The parts' rows lie at rows + warp * kStride + row * kPitch
+// (floats), or in the spill of the warp.
+template <typename T, int kWarps, int kRows, int kStride, int kPitch, int kWidth>
+__device__ __forceinline__ void paged_merge(const PagedArgs& a, const PagedParts<kWarps, kRows>& parts,
+                                            const float* rows) {
+  static_assert(kWarps <= 16, "a lane for each part");
+  const int lane = threadIdx.x & 31;
+  bool present = false, starts = false;
+  if (lane < 2 * kWarps) {
+    const PartRecord& r = parts.records[lane >> 1][lane & 1];
+    present = !r.empty();
+    starts = starts_unit(r, lane & 1);
+  }
+  const uint32_t all = __ballot_sync(kFullMask, present);
+  const uint32_t first = __ballot_sync(kFullMask, starts);
+  const int pieces = a.head_dim / kWidth;
+  // A few units: all threads on each.  Many, of short sequences: a warp each.
+  const bool together = __popc(first) <= 2;
+  int turn = 0;
+  for (uint32_t left = first; left != 0; left &= left - 1, ++turn) {
+    if (!together && turn % kWarps != static_cast<int>(threadIdx.x >> 5)) continue;
+    const int start = __ffs(left) - 1;
+    const uint32_t mine = parts_of_unit(all, first, start);
+    const int last = 31 - __clz(mine);
+    const PartRecord& r = parts.records[start >> 1][start & 1];
+    const bool whole = r.begin == 0 && parts.records[last >> 1][last & 1].end == r.tiles;
+    const PagedUnit unit = paged_unit<kRows>(a, r.unit);
+    for (int i = together ? threadIdx.x : lane; i < unit.rows * pieces;
+         i += together ? 32 * kWarps : 32) {
+      const int row = i / pieces, d = (i - row * pieces) * kWidth;
+      // A warp has one part of a unit: the loads do not wait for one another.
+      float m[kWarps], l[kWarps], v[kWarps][kWidth];
+#pragma unroll
+      for (int b = 0; b < kWarps; ++b) {
+        m[b] = -INFINITY, l[b] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < kWidth; ++e) v[b][e] = 0.0f;
+        const uint32_t kinds = mine >> (2 * b) & 3u;
+        if (kinds == 0) continue;
+        const int kind = kinds == 1u << kTail ? kTail : kHead;
+        m[b] = parts.m[b][kind][row];
+        l[b] = parts.l[b][kind][row];
+        if (parts.records[b][kind].spilled == 0)
+          ld_row(rows + b * kStride + row * kPitch + d, false, v[b]);
+        else
+          ld_row(a.spill + ((static_cast<int64_t>(blockIdx.x) * kWarps + b) * a.row_cap + row) *
+                               a.head_dim + d,
+                 true, v[b]);
+      }
+      float top = m[0];
+#pragma unroll
+      for (int b = 1; b < kWarps; ++b) top = fmaxf(top, m[b]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f, out[kWidth] = {};
+#pragma unroll
+      for (int b = 0; b < kWarps; ++b) {
+        const float f = paged_exp2(m[b] - base);
+        sum = fmaf(f, l[b], sum);
+#pragma unroll
+        for (int e = 0; e < kWidth; ++e) out[e] = fmaf(f, v[b][e], out[e]);
+      }
+      if (whole) {
+#pragma unroll
+        for (int e = 0; e < kWidth; ++e) out[e] /= sum;
+        st_row(static_cast<T*>(a.out) +
+                   (static_cast<int64_t>(r.sequence) * a.heads + unit.first_head + row) * a.head_dim + d,
+               out);
+      } else {
+        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (r.begin == 0 ? 1 : 0);
+        st_row(a.partial + (slot * a.row_cap + row) * a.head_dim + d, out);
+        if (d == 0) a.partial_ml[slot * a.row_cap + row] = make_float2(top, sum);
+      }
+    }
+  }
+}
+
+// Joins the parts of the unit that CTA blockIdx.x of the main launch starts
+// and does not end (slot 1 of that CTA, slot 0 of the following ones), row
+// blockIdx.y, in key order: warp w takes parts w, w + 8, ...
+constexpr int kJoinThreads = 256;
+
+template <typename T, int kUnitTile, int kUnitWarps, int kRows, int kWidth>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a, int grid_ctas) {
+  constexpr int kJoinWarps = kJoinThreads / 32;
+  constexpr int kHeld = kPagedMaxHeadDim / (32 * kWidth);  // pieces of a lane
+  __shared__ PagedStart found[1];
+  __shared__ float warp_top[kJoinWarps], warp_sum[kJoinWarps];
+  __shared__ float rows[kJoinWarps][kPagedMaxHeadDim];
+  pdl_begin();
+  const int cta = blockIdx.x;
+  const auto cta_begin = [](const PagedTotal& t, int64_t index) {
+    return t.ranges.begin(kUnitWarps * index);
+  };
+  const PagedTotal total = paged_start<kJoinThreads, kUnitTile, kUnitWarps>(
+      a, grid_ctas, found, [&](const PagedTotal& t, int) -> long long {
+        return cta + 1 < t.ctas ? cta_begin(t, cta + 1) - 1 : -1;
+      });
+  if (cta + 1 >= total.ctas) return;
+  const int64_t at = cta_begin(total, cta + 1) - 1;  // the CTA's last tile
+  const int sequence = found[0].sequence;
+  const int tiles = key_tiles(paged_length(a, sequence), kUnitTile);
+  const TilePlace last = place_of(at, found[0].before, tiles, a.units.divisor);
+  if (last.tile + 1 == tiles) return;  // not cut here
+  const int64_t unit_begin = at - last.tile;
+  if (unit_begin < cta_begin(total, cta)) return;  // an earlier CTA starts it
+  const PagedUnit unit = paged_unit<kRows>(a, last.unit);
+  const int row = blockIdx.y;
+  if (row >= unit.rows) return;
+  const int parts =
+      static_cast<int>(total.ranges.holder(unit_begin + tiles - 1) / kUnitWarps) - cta + 1;
+  const auto part_row = [&](int p) {
+    const int64_t slot = p == 0 ? 2 * static_cast<int64_t>(cta) + 1 : 2 * static_cast<int64_t>(cta + p);
+    return slot * a.row_cap + row;
+  };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float top = -INFINITY;
+  for (int p = threadIdx.x; p < parts; p += kJoinThreads)
+    top = fmaxf(top, __ldcg(&a.partial_ml[part_row(p)]).x);
+  top = warp_max(top);
+  if (lane == 0) warp_top[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, warp_top[w]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f, out[kHeld][kWidth] = {};
+#pragma unroll 4
+  for (int p = warp; p < parts; p += kJoinWarps) {
+    const float2 ml = __ldcg(&a.partial_ml[part_row(p)]);
+    const float f = paged_exp2(ml.x - base);
+    sum = fmaf(f, ml.y, sum);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int d = (32 * i + lane) * kWidth;
+      if (d >= a.head_dim) continue;
+      float v[kWidth];
+      ld_row(a.partial + part_row(p) * a.head_dim + d, true, v);
+#pragma unroll
+      for (int e = 0; e < kWidth; ++e) out[i][e] = fmaf(f, v[e], out[i][e]);
+    }
+  }
+  if (lane == 0) warp_sum[warp] = sum;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+#pragma unroll
+    for (int e = 0; e < kWidth; ++e) rows[warp][(32 * i + lane) * kWidth + e] = out[i][e];
+  __syncthreads();
+  for (int d = threadIdx.x; d < a.head_dim; d += kJoinThreads) {
+    float l = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) l += warp_sum[w], o += rows[w][d];
+    st_out(static_cast<T*>(a.out) +
+               (static_cast<int64_t>(sequence) * a.heads + unit.first_head + row) * a.head_dim + d,
+           o / l);
+  }
+}
+
+template <typename T, int kUnitTile, int kUnitWarps, int kRows>
+cudaError_t launch_join(const PagedArgs& a, int grid_ctas, cudaStream_t stream) {
+  const dim3 grid(grid_ctas - 1, a.row_cap), block(kJoinThreads);
+  if (a.head_dim % 4 == 0)
+    return launch_pdl(paged_join_kernel<T, kUnitTile, kUnitWarps, kRows, 4>, grid, block, stream, a,
+                      grid_ctas);
+  return launch_pdl(paged_join_kernel<T, kUnitTile, kUnitWarps, kRows, 1>, grid, block, stream, a,
+                    grid_ctas);
 }
 
 // The most CTAs of a launch; the workspace is sized for them.
@@ -198,15 +357,34 @@ inline int paged_grid_limit() { return 2 * sm_count(); }
 
 // CTAs of a launch: at most `limit`, and no more than the longest batch that
 // the block table can hold keeps busy.
-inline int paged_grid(const PagedArgs& a, int limit, int tile, int least, int unit_rows) {
+inline int paged_grid(const PagedArgs& a, int limit, int tile, int warps, int unit_rows) {
   const int64_t capacity = static_cast<int64_t>(a.max_pages) * a.page_size.divisor;
   const int64_t tiles = capacity <= tile ? 1 : (capacity - 1) / tile + 1;
   const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads *
                         ((a.group + unit_rows - 1) / unit_rows);
   // The product may pass 63 bits; then only its comparison with the limit counts.
   const double total = static_cast<double>(tiles) * static_cast<double>(units);
-  if (total >= static_cast<double>(limit) * least) return limit;
-  return active_ctas(tiles * units, limit, least);
+  if (total >= static_cast<double>(limit) * warps) return limit;
+  return active_ctas(tiles * units, limit, warps);
+}
+
+constexpr int kPagedMaxRows = 16, kPagedMaxWarps = 8;
+
+// Lays the scratch out; its size is that of the largest launch.
+inline void paged_scratch(PagedArgs* a, int grid, int warps, int rows) {
+  a->parts = make_fast_div((a->group + rows - 1) / rows);
+  a->units = make_fast_div(a->kv_heads * a->parts.divisor);
+  a->row_cap = a->group < rows ? a->group : rows;
+  const int64_t slots = static_cast<int64_t>(grid) * 2 * a->row_cap;
+  a->spill = a->partial + slots * a->head_dim;
+  a->partial_ml = reinterpret_cast<float2*>(
+      a->spill + static_cast<int64_t>(grid) * warps * a->row_cap * a->head_dim);
+}
+
+inline size_t paged_scratch_bytes(int group, int head_dim) {
+  const size_t rows = group < kPagedMaxRows ? group : kPagedMaxRows;
+  const size_t ctas = paged_grid_limit();
+  return ctas * rows * ((2 + kPagedMaxWarps) * sizeof(float) * head_dim + 2 * sizeof(float2));
 }
 
 // The tensor-core kernel: 16-bit types, head_dim a multiple of 8, addresses

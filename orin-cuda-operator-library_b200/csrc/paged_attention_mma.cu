@@ -48,9 +48,6 @@ namespace opl {
 namespace {
 
 constexpr int kTile = 16;
-// Block-table entries are loaded this many steps before their copies.
-constexpr int kAhead = 2;
-
 template <typename T>
 struct Mma;
 template <>
@@ -140,15 +137,16 @@ struct MapOrder {
 };
 
 // Copies are made by the TMA unit, or by the lanes (kTma false).
-template <typename T, int kDim, int kRows, bool kTma, int kWarps, int kStages, int kLeast>
+template <typename T, int kDim, int kRows, bool kTma, int kWarps, int kStages>
 __global__ void __launch_bounds__(32 * kWarps, 1)
     paged_mma_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap k_map,
-                     const __grid_constant__ CUtensorMap v_map, const MapOrder order, int row_cap) {
+                     const __grid_constant__ CUtensorMap v_map, const MapOrder order) {
   using S = Shape<T, kDim, kRows, kWarps, kStages>;
   constexpr int kThreads = 32 * kWarps;
   constexpr int kHalves = kRows / 8;  // row groups of the S accumulator in use
   extern __shared__ unsigned char shared[];
-  __shared__ float merge_m[kWarps][kRows], merge_l[kWarps][kRows];
+  __shared__ PagedParts<kWarps, kRows> parts;
+  __shared__ PagedStart starts[kWarps];
   __shared__ uint64_t full[kWarps][kStages];
   __shared__ int abort_wait;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -172,337 +170,416 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
 
   const T* q = static_cast<const T*>(a.q);
   const int page_size = static_cast<int>(a.page_size.divisor);
+  if (lane < 2) parts.records[warp][lane] = PartRecord{};
   // The barriers are also set up before the first copy by this search's
   // __syncthreads.
-  const PagedStart start = paged_start<kThreads, kTile, kLeast>(
-      a, gridDim.x, [](long long total, int ctas) -> long long {
-        return static_cast<int>(blockIdx.x) < ctas ? range_begin(total, ctas, blockIdx.x) : -1;
+  const PagedTotal total = paged_start<kThreads, kTile, kWarps>(
+      a, gridDim.x, starts, [](const PagedTotal& x, int target) -> long long {
+        return static_cast<int>(blockIdx.x) < x.ctas
+                   ? x.ranges.begin(int64_t{kWarps} * blockIdx.x + target)
+                   : -1;
       });
-  if (static_cast<int>(blockIdx.x) >= start.ctas) return;
-  int64_t w = range_begin(start.total, start.ctas, blockIdx.x);
-  const int64_t limit = range_begin(start.total, start.ctas, blockIdx.x + 1);
-  int sequence = start.sequence;
-  int64_t before = start.before;
+  if (static_cast<int>(blockIdx.x) >= total.ctas) return;
+  const int64_t range = int64_t{kWarps} * blockIdx.x + warp;
+  const int64_t w = total.ranges.begin(range);
+  const bool opens = w == total.ranges.begin(int64_t{kWarps} * blockIdx.x);
+  int64_t to_fetch = total.ranges.begin(range + 1) - w, to_read = to_fetch;
   int reported = 0;
   int slot_in = 0, slot_out = 0;  // ring stages being filled and read
   uint32_t parity = 0;            // of the stage being read
-  bool dead = false;              // a wait gave up; the warp copies no more
 
   // Where this lane's pieces lie in a stage (see the layout above).
   const uint32_t k_piece = g * 128 + (2 * t ^ g) * 16;
   const uint32_t v_piece = S::kKeyBytes + 2 * t * 128 + (g ^ 2 * t) * 16;
   const uint32_t ring_address = tc::smem_u32(ring);
 
-  while (w < limit) {
-    const int raw_length = ld_int(a.seq_lens + sequence);
-    const int length = readable_length(raw_length, a.max_pages, page_size);
-    if (length != raw_length) reported = kBadLength;
-    const int tiles = key_tiles(length, kTile);
-    if (w >= (before + tiles) * a.units()) {
-      before += tiles;
-      ++sequence;
-      continue;
+  // Two cursors walk over the warp's tiles: `in`, the next one to be fetched,
+  // and `out`, the one being read.  The length of the next sequence is loaded
+  // while this one lasts.
+  struct Cursor {
+    int sequence, unit, tile, tiles, length, next_length;
+  };
+  const int units = static_cast<int>(a.units.divisor);
+  const auto load_length = [&](int sequence) {
+    return sequence < a.batch ? ld_int(a.seq_lens + sequence) : 0;
+  };
+  const auto enter = [&](Cursor& c, int raw) {
+    c.length = readable_length(raw, a.max_pages, page_size);
+    if (c.length != raw) reported = kBadLength;
+    c.tiles = key_tiles(c.length, kTile);
+    c.next_length = load_length(c.sequence + 1);
+  };
+  const auto advance = [&](Cursor& c) {
+    if (++c.tile < c.tiles) return;
+    c.tile = 0;
+    if (++c.unit < units) return;
+    c.unit = 0;
+    ++c.sequence;
+    enter(c, c.next_length);
+  };
+  Cursor in = {};
+  if (to_read > 0) {
+    in.sequence = starts[warp].sequence;
+    enter(in, load_length(in.sequence));
+    const TilePlace p = place_of(w, starts[warp].before, in.tiles, units);
+    in.unit = p.unit;
+    in.tile = p.tile;
+  }
+  Cursor out = in;
+
+  // The key that this lane places in a tile: with the TMA unit the first of a
+  // box of 16 or 8 (even and odd lanes: first and second half of the tile),
+  // else lanes 0-15 a key each and lanes 16-31 their values.  Its block-table
+  // entry is loaded a step before the tile is copied.
+  struct Fetched {
+    int first, length, kv_head;  // of the tile; length < 0: no tile
+    int page;                    // of this lane's key
+  };
+  const int key_offset = kTma ? 8 * (lane & 1) : lane & 15;
+  const auto fetch = [&]() {
+    Fetched f = {0, -1, 0, 0};
+    if (to_fetch > 0) {
+      --to_fetch;
+      f.first = in.tile * kTile;
+      f.length = in.length;
+      f.kv_head = static_cast<int>(fast_div(in.unit, a.parts));
+      const int key = f.first + key_offset;
+      if (key < in.length)
+        f.page = ld_int(a.block_table + in.sequence * a.table_row + fast_div(key, a.page_size));
+      advance(in);
     }
-    const Segment segment = segment_at(w, limit, before, tiles, a.units());
-    w += segment.end - segment.begin;
-    const PagedUnit unit = paged_unit<kRows>(a, segment.unit);
-    const int* table = a.block_table + sequence * a.table_row;
-    const int first = segment.begin + warp;
-    const int count = !dead && first < segment.end ? (segment.end - first - 1) / kWarps + 1 : 0;
-
-    // The key that this lane places in tile i: with the TMA unit the first of
-    // a box of 16 or 8 (even and odd lanes: first and second half of the
-    // tile), else lanes 0-15 a key each and lanes 16-31 their values.  Its
-    // block-table entry is loaded some steps before it is used.
-    const auto key_of = [&](int i) {
-      return (first + i * kWarps) * kTile + (kTma ? 8 * (lane & 1) : lane & 15);
-    };
-    const auto fetch = [&](int i) {
-      const int key = key_of(i);
-      return i < count && key < length ? ld_int(table + fast_div(key, a.page_size)) : 0;
-    };
-    // Copies tile i into the next stage; bit j of the result: key j is there.
-    const auto issue = [&](int i, int page) -> uint32_t {
-      uint32_t there = 0;
-      if (i < count) {
-        const int key = key_of(i);
-        const bool known = key < length;
-        const bool ok = known && cache_page(page, a.pages);
-        if (known && !ok) reported = kBadPage;
-        const int inside = key - static_cast<int>(fast_div(key, a.page_size)) * page_size;
-        if constexpr (kTma) {
-          const uint32_t halves = __ballot_sync(kFullMask, ok) & 3u;
-          const int left = length - (first + i * kWarps) * kTile;
-          there = left >= kTile ? 0xffffu : (1u << left) - 1;
-          if ((halves & 1u) == 0) there &= 0xff00u;
-          if ((halves & 2u) == 0) there &= 0x00ffu;
-          uint64_t* const bar = &full[warp][slot_in];
-          if (lane == 0) tc::mbar_expect_tx(bar, S::kStageBytes);
-          __syncwarp();
-          if (lane < order.boxes) {
-            // A box that holds no key lies past the last page: zeros.
-            const int p = ok ? page : static_cast<int>(a.pages);
-            const int y = order.token_first ? inside : unit.kv_head;
-            const int z = order.token_first ? unit.kv_head : inside;
-            unsigned char* dst = ring + slot_in * S::kStageBytes + lane * 1024;
+    return f;
+  };
+  // Copies a tile into the next stage; bit j of the result: key j is there.
+  const auto issue = [&](const Fetched& f) -> uint32_t {
+    uint32_t there = 0;
+    if (f.length >= 0) {
+      const int key = f.first + key_offset;
+      const bool known = key < f.length;
+      const bool ok = known && cache_page(f.page, a.pages);
+      if (known && !ok) reported = kBadPage;
+      const int inside = key - static_cast<int>(fast_div(key, a.page_size)) * page_size;
+      if constexpr (kTma) {
+        const uint32_t halves = __ballot_sync(kFullMask, ok) & 3u;
+        const int left = f.length - f.first;
+        there = left >= kTile ? 0xffffu : (1u << left) - 1;
+        if ((halves & 1u) == 0) there &= 0xff00u;
+        if ((halves & 2u) == 0) there &= 0x00ffu;
+        uint64_t* const bar = &full[warp][slot_in];
+        if (lane == 0) tc::mbar_expect_tx(bar, S::kStageBytes);
+        __syncwarp();
+        if (lane < order.boxes) {
+          // A box that holds no key lies past the last page: zeros.
+          const int p = ok ? f.page : static_cast<int>(a.pages);
+          const int y = order.token_first ? inside : f.kv_head;
+          const int z = order.token_first ? f.kv_head : inside;
+          unsigned char* dst = ring + slot_in * S::kStageBytes + lane * 1024;
 #pragma unroll
-            for (int c = 0; c < kDim / 64; ++c)
-              tc::tma_load_4d(dst + c * 2048, &k_map, 64 * c, y, z, p, bar);
+          for (int c = 0; c < kDim / 64; ++c)
+            tc::tma_load_4d(dst + c * 2048, &k_map, 64 * c, y, z, p, bar);
 #pragma unroll
-            for (int c = 0; c < kDim / 64; ++c)
-              tc::tma_load_4d(dst + S::kKeyBytes + c * 2048, &v_map, 64 * c, y, z, p, bar);
-          }
-        } else {
-          const int64_t place = !ok ? -1
-                                : lane < 16
-                                    ? page * a.k_page + inside * a.k_token + unit.kv_head * a.k_head
-                                    : page * a.v_page + inside * a.v_token + unit.kv_head * a.v_head;
-          there = __ballot_sync(kFullMask, ok) & 0xffffu;
-          // Eight lanes copy 128 bytes of one row.
-          const int piece = lane & 7;
-          uint32_t dst = ring_address + slot_in * S::kStageBytes;
-#pragma unroll
-          for (int s = 0; s < 8; ++s) {
-            const int row = 4 * (s & 3) + (lane >> 3);
-            const int64_t at = __shfl_sync(kFullMask, place, (s < 4 ? 0 : 16) + row);
-            const T* const src =
-                static_cast<const T*>(s < 4 ? a.k : a.v) + (at >= 0 ? at : 0) + 8 * piece;
-            const uint32_t to = dst + row * 128 + (piece ^ (row & 7)) * 16;
-#pragma unroll
-            for (int c = 0; c < kDim / 64; ++c)
-              copy16(to + (s < 4 ? 0 : S::kKeyBytes) + c * 2048, src + 64 * c,
-                     at >= 0 && 64 * c + 8 * piece < a.head_dim);
-          }
+          for (int c = 0; c < kDim / 64; ++c)
+            tc::tma_load_4d(dst + S::kKeyBytes + c * 2048, &v_map, 64 * c, y, z, p, bar);
         }
-        if (++slot_in == kStages) slot_in = 0;
+      } else {
+        const int64_t place =
+            !ok         ? -1
+            : lane < 16 ? f.page * a.k_page + inside * a.k_token + f.kv_head * a.k_head
+                        : f.page * a.v_page + inside * a.v_token + f.kv_head * a.v_head;
+        there = __ballot_sync(kFullMask, ok) & 0xffffu;
+        // Eight lanes copy 128 bytes of one row.
+        const int piece = lane & 7;
+        const uint32_t dst = ring_address + slot_in * S::kStageBytes;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          const int row = 4 * (s & 3) + (lane >> 3);
+          const int64_t at = __shfl_sync(kFullMask, place, (s < 4 ? 0 : 16) + row);
+          const T* const src =
+              static_cast<const T*>(s < 4 ? a.k : a.v) + (at >= 0 ? at : 0) + 8 * piece;
+          const uint32_t to = dst + row * 128 + (piece ^ (row & 7)) * 16;
+#pragma unroll
+          for (int c = 0; c < kDim / 64; ++c)
+            copy16(to + (s < 4 ? 0 : S::kKeyBytes) + c * 2048, src + 64 * c,
+                   at >= 0 && 64 * c + 8 * piece < a.head_dim);
+        }
       }
-      if constexpr (!kTma) copy_commit();
-      return there;
-    };
+      if (++slot_in == kStages) slot_in = 0;
+    }
+    if constexpr (!kTma) copy_commit();
+    return there;
+  };
 
-    uint32_t there[kStages];
-    int pages[kStages - 1 + kAhead];
+  uint32_t there[kStages];
+  Fetched fetched;
+  {
+    Fetched early[kStages - 1];
 #pragma unroll
-    for (int i = 0; i < kStages - 1 + kAhead; ++i) pages[i] = fetch(i);
+    for (int i = 0; i < kStages - 1; ++i) early[i] = fetch();
+    fetched = fetch();
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) there[i] = issue(i, pages[i]);
+    for (int i = 0; i < kStages - 1; ++i) there[i] = issue(early[i]);
+  }
 
-    // Q in the order of the key pieces: words 0, 1 of piece j are the first
-    // instruction's two k pairs, words 2, 3 the second's.
-    uint4 qa[kDim / 32][kHalves];
+  // Q in the order of the key pieces: words 0, 1 of piece j are the first
+  // instruction's two k pairs, words 2, 3 the second's.  The next segment's is
+  // loaded during this one, where registers allow.
+  constexpr bool kQueryAhead = kDim * kRows <= 1024;
+  using Query = uint4[kDim / 32][kHalves];
+  Query qa, q_next;
+  const auto load_query = [&](Query& x, int sequence, int unit) {
+    const PagedUnit u = paged_unit<kRows>(a, unit);
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       const int row = g + 8 * h;
-      const T* src = q + sequence * a.q_batch + (unit.first_head + row) * a.q_head;
+      const T* src = q + sequence * a.q_batch + (u.first_head + row) * a.q_head;
 #pragma unroll
       for (int j = 0; j < kDim / 32; ++j) {
         const int d = 64 * (j / 2) + 16 * t + 8 * (j & 1);
-        qa[j][h] = row < unit.rows && d < a.head_dim ? ld_ro(reinterpret_cast<const uint4*>(src + d))
-                                                     : make_uint4(0, 0, 0, 0);
+        x[j][h] = row < u.rows && d < a.head_dim ? ld_ro(reinterpret_cast<const uint4*>(src + d))
+                                                 : make_uint4(0, 0, 0, 0);
       }
     }
-    float o[kDim / 8][4];
+  };
+  const auto load_next_query = [&]() {
+    const bool same = out.unit + 1 < units;
+    if (same || out.sequence + 1 < a.batch)
+      load_query(q_next, same ? out.sequence : out.sequence + 1, same ? out.unit + 1 : 0);
+  };
+  float o[kDim / 8][4];
+  float m[kHalves], l[kHalves];  // l over this lane's keys only
+  const auto clear = [&]() {
 #pragma unroll
     for (int n = 0; n < kDim / 8; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
-    float m[kHalves], l[kHalves];  // l over this lane's keys only
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) m[h] = -INFINITY, l[h] = 0.0f;
+  };
+  clear();
+  int begin = out.tile;  // of the segment
+  if (to_read > 0) {
+    load_query(qa, out.sequence, out.unit);
+    if constexpr (kQueryAhead) load_next_query();
+  }
 
-    for (int i = 0; i < count; ++i) {
-      const int later_page = fetch(i + kStages - 1 + kAhead);
-      __syncwarp();  // every lane has read the stage that is filled next
-      there[kStages - 1] = issue(i + kStages - 1, pages[kStages - 1]);
-#pragma unroll
-      for (int x = kStages - 1; x < kStages - 2 + kAhead; ++x) pages[x] = pages[x + 1];
-      pages[kStages - 2 + kAhead] = later_page;
-      if constexpr (kTma) {
-        if (!tc::mbar_wait_warp(&full[warp][slot_out], parity, &abort_wait, a.watchdog,
-                                tc::kWatchdogPaged)) {
-          // Give the other copies in flight the same time to land, then leave
-          // the segment; the output is not valid and the watchdog says so.
-          for (int x = 1; x < kStages && i + x < count; ++x) {
-            const int slot = (slot_out + x) % kStages;
-            volatile int alone = 0;
-            tc::mbar_wait(&full[warp][slot], slot < slot_out ? parity ^ 1u : parity, &alone,
-                          a.watchdog, tc::kWatchdogPaged);
-          }
-          dead = true;
-          break;
+  while (to_read > 0) {
+    __syncwarp();  // every lane has read the stage that is filled next
+    there[kStages - 1] = issue(fetched);
+    fetched = fetch();
+    if constexpr (kTma) {
+      if (!tc::mbar_wait_warp(&full[warp][slot_out], parity, &abort_wait, a.watchdog,
+                              tc::kWatchdogPaged)) {
+        // Give the other copies in flight the same time to land and stop; the
+        // output is not valid and the watchdog says so.
+        for (int x = 1; x < kStages && x < to_read; ++x) {
+          const int slot = (slot_out + x) % kStages;
+          volatile int alone = 0;
+          tc::mbar_wait(&full[warp][slot], slot < slot_out ? parity ^ 1u : parity, &alone,
+                        a.watchdog, tc::kWatchdogPaged);
         }
-      } else {
-        copy_wait<kStages - 1>();
-        __syncwarp();  // what the other lanes copied
+        break;
       }
-      const uint32_t stage = ring_address + slot_out * S::kStageBytes;
-      if (++slot_out == kStages) slot_out = 0, parity ^= 1u;
+    } else {
+      copy_wait<kStages - 1>();
+      __syncwarp();  // what the other lanes copied
+    }
+    const uint32_t stage = ring_address + slot_out * S::kStageBytes;
+    if (++slot_out == kStages) slot_out = 0, parity ^= 1u;
 
-      float s[2][4] = {};
+    float s[2][4] = {};
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int j = 0; j < kDim / 32; ++j) {
+        const uint4 b = ld_shared(stage + (k_piece ^ (j & 1) * 16) + (j / 2) * 2048 + n * 1024);
+        Mma<T>::run(s[n], qa[j][0].x, kHalves == 2 ? qa[j][kHalves - 1].x : 0u, qa[j][0].y,
+                    kHalves == 2 ? qa[j][kHalves - 1].y : 0u, b.x, b.y);
+        Mma<T>::run(s[n], qa[j][0].z, kHalves == 2 ? qa[j][kHalves - 1].z : 0u, qa[j][0].w,
+                    kHalves == 2 ? qa[j][kHalves - 1].w : 0u, b.z, b.w);
+      }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int x = 0; x < 2 * kHalves; ++x) s[n][x] *= a.scale_log2;
+    const uint32_t seen = there[0];
+    if (seen != 0xffffu) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int j = 0; j < kDim / 32; ++j) {
-          const uint4 b = ld_shared(stage + (k_piece ^ (j & 1) * 16) + (j / 2) * 2048 + n * 1024);
-          Mma<T>::run(s[n], qa[j][0].x, kHalves == 2 ? qa[j][kHalves - 1].x : 0u, qa[j][0].y,
-                      kHalves == 2 ? qa[j][kHalves - 1].y : 0u, b.x, b.y);
-          Mma<T>::run(s[n], qa[j][0].z, kHalves == 2 ? qa[j][kHalves - 1].z : 0u, qa[j][0].w,
-                      kHalves == 2 ? qa[j][kHalves - 1].w : 0u, b.z, b.w);
-        }
+        for (int x = 0; x < 2 * kHalves; ++x)
+          if ((seen >> (8 * n + 2 * t + (x & 1)) & 1u) == 0) s[n][x] = -INFINITY;
+    }
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int x = 0; x < 2 * kHalves; ++x) s[n][x] *= a.scale_log2;
-      const uint32_t seen = there[0];
-      if (seen != 0xffffu) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int x = 0; x < 2 * kHalves; ++x)
-            if ((seen >> (8 * n + 2 * t + (x & 1)) & 1u) == 0) s[n][x] = -INFINITY;
-      }
-#pragma unroll
-      for (int x = 0; x + 1 < kStages; ++x) there[x] = there[x + 1];
+    for (int x = 0; x + 1 < kStages; ++x) there[x] = there[x + 1];
 
-      float m_new[kHalves];
-      bool moved = false;
+    float m_new[kHalves];
+    bool moved = false;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+      top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
+      m_new[h] = fmaxf(m[h], top);
+      moved |= m_new[h] != m[h];
+    }
+    float base[kHalves];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+      base[h] = m_new[h] == -INFINITY ? 0.0f : m_new[h];  // no key so far: all weights 0
+    if (__any_sync(kFullMask, moved)) {
+      float alpha[kHalves];
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
-        float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-        top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
-        m_new[h] = fmaxf(m[h], top);
-        moved |= m_new[h] != m[h];
+        alpha[h] = paged_exp2(m[h] - base[h]);
+        l[h] *= alpha[h];
+        m[h] = m_new[h];
       }
-      float base[kHalves];
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h)
-        base[h] = m_new[h] == -INFINITY ? 0.0f : m_new[h];  // no key so far: all weights 0
-      if (__any_sync(kFullMask, moved)) {
-        float alpha[kHalves];
+      for (int n = 0; n < kDim / 8; ++n)
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          alpha[h] = paged_exp2(m[h] - base[h]);
-          l[h] *= alpha[h];
-          m[h] = m_new[h];
-        }
+        for (int x = 0; x < 4; ++x) o[n][x] *= alpha[kHalves == 2 ? x >> 1 : 0];
+    }
+    uint32_t p[2][kHalves], rest[2][kHalves];
 #pragma unroll
-        for (int n = 0; n < kDim / 8; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[n][x] *= alpha[kHalves == 2 ? x >> 1 : 0];
+      for (int h = 0; h < kHalves; ++h) {
+        const float x = paged_exp2(s[n][2 * h] - base[h]);
+        const float y = paged_exp2(s[n][2 * h + 1] - base[h]);
+        l[h] += x + y;
+        p[n][h] = Mma<T>::split(x, y, &rest[n][h]);
       }
-      uint32_t p[2][kHalves], rest[2][kHalves];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+    for (int c = 0; c < kDim / 64; ++c) {
+      uint4 v[4];
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          const float x = paged_exp2(s[n][2 * h] - base[h]);
-          const float y = paged_exp2(s[n][2 * h + 1] - base[h]);
-          l[h] += x + y;
-          p[n][h] = Mma<T>::split(x, y, &rest[n][h]);
+      for (int x = 0; x < 4; ++x)  // keys 2t, 2t + 1, 2t + 8, 2t + 9
+        v[x] = ld_shared(stage + (x & 1 ? (v_piece ^ 16) + 128 : v_piece) + c * 2048 +
+                         (x >> 1) * 1024);
+      if (seen != 0xffffu) {  // what lies behind the length is not a value
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if ((seen >> (2 * t + (x & 1) + 8 * (x >> 1)) & 1u) == 0) v[x] = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint32_t b0, b1;
+        if (e & 1) {
+          b0 = pair_halves<true>(word(v[0], e / 2), word(v[1], e / 2));
+          b1 = pair_halves<true>(word(v[2], e / 2), word(v[3], e / 2));
+        } else {
+          b0 = pair_halves<false>(word(v[0], e / 2), word(v[1], e / 2));
+          b1 = pair_halves<false>(word(v[2], e / 2), word(v[3], e / 2));
         }
-#pragma unroll
-      for (int c = 0; c < kDim / 64; ++c) {
-        uint4 v[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x)  // keys 2t, 2t + 1, 2t + 8, 2t + 9
-          v[x] = ld_shared(stage + (x & 1 ? (v_piece ^ 16) + 128 : v_piece) + c * 2048 +
-                           (x >> 1) * 1024);
-        if (seen != 0xffffu) {  // what lies behind the length is not a value
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if ((seen >> (2 * t + (x & 1) + 8 * (x >> 1)) & 1u) == 0) v[x] = make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          uint32_t b0, b1;
-          if (e & 1) {
-            b0 = pair_halves<true>(word(v[0], e / 2), word(v[1], e / 2));
-            b1 = pair_halves<true>(word(v[2], e / 2), word(v[3], e / 2));
-          } else {
-            b0 = pair_halves<false>(word(v[0], e / 2), word(v[1], e / 2));
-            b1 = pair_halves<false>(word(v[2], e / 2), word(v[3], e / 2));
-          }
-          if constexpr (kHalves == 1) {
-            Mma<T>::run(o[8 * c + e], p[0][0], rest[0][0], p[1][0], rest[1][0], b0, b1);
-          } else {
-            Mma<T>::run(o[8 * c + e], p[0][0], p[0][kHalves - 1], p[1][0], p[1][kHalves - 1], b0,
-                        b1);
-            Mma<T>::run(o[8 * c + e], rest[0][0], rest[0][kHalves - 1], rest[1][0],
-                        rest[1][kHalves - 1], b0, b1);
-          }
+        if constexpr (kHalves == 1) {
+          Mma<T>::run(o[8 * c + e], p[0][0], rest[0][0], p[1][0], rest[1][0], b0, b1);
+        } else {
+          Mma<T>::run(o[8 * c + e], p[0][0], p[0][kHalves - 1], p[1][0], p[1][kHalves - 1], b0,
+                      b1);
+          Mma<T>::run(o[8 * c + e], rest[0][0], rest[0][kHalves - 1], rest[1][0],
+                      rest[1][kHalves - 1], b0, b1);
         }
       }
     }
-    if constexpr (!kTma) copy_wait<0>();
 
-    // Merge the warps, each through its own (now empty) ring.
+    --to_read;
+    if (out.tile + 1 < out.tiles && to_read > 0) {
+      ++out.tile;
+      continue;
+    }
+
+    // The segment ends.
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       l[h] += __shfl_xor_sync(kFullMask, l[h], 1);
       l[h] += __shfl_xor_sync(kFullMask, l[h], 2);
-      if (t == 0) {
-        merge_m[warp][g + 8 * h] = m[h];
-        merge_l[warp][g + 8 * h] = l[h];
-      }
     }
-    __syncwarp();  // the ring is written across lanes from here
-    float* const merge_o = reinterpret_cast<float*>(ring);
+    if constexpr (kHalves == 1) {
+      // An infinite value times a rest of zero is no number; the first part of
+      // the weight alone gives the infinity.
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h)
+      for (int n = 0; n < kDim / 8; ++n)
 #pragma unroll
-      for (int c = 0; c < kDim / 64; ++c)
+        for (int x = 0; x < 2; ++x)
+          if (o[n][2 + x] == o[n][2 + x]) o[n][x] += o[n][2 + x];
+    }
+    const PagedUnit unit = paged_unit<kRows>(a, out.unit);
+    // The lane's rows are g + 8h; of piece c it holds columns 8 (2t + x) + e in
+    // o[8c + e][2h + x].
+    if (begin == 0 && out.tile + 1 == out.tiles) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)  // columns 8 (2t + x) + e of the piece
+      for (int h = 0; h < kHalves; ++h) {
+        const int row = g + 8 * h;
+        const float f = out.length == 0 ? 0.0f : 1.0f / l[h];
+        T* const dst =
+            static_cast<T*>(a.out) +
+            (static_cast<int64_t>(out.sequence) * a.heads + unit.first_head + row) * a.head_dim;
 #pragma unroll
-          for (int e = 0; e < 8; e += 4) {
-            float4 out;
-            float* const f = &out.x;
+        for (int c = 0; c < kDim / 64; ++c)
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const float (&acc)[4] = o[8 * c + e + y];
-              if constexpr (kHalves == 1) {
-                // An infinite value times a rest of zero is no number; the
-                // first part of the weight alone gives the infinity.
-                f[y] = acc[2 + x] == acc[2 + x] ? acc[x] + acc[2 + x] : acc[x];
-              } else {
-                f[y] = acc[2 * h + x];
-              }
-            }
-            *reinterpret_cast<float4*>(merge_o + (g + 8 * h) * S::kPitch + 64 * c + 8 * (2 * t + x) +
-                                       e) = out;
+          for (int x = 0; x < 2; ++x) {
+            const int d = 64 * c + 8 * (2 * t + x);
+            alignas(16) T y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) st_out(&y[e], o[8 * c + e][2 * h + x] * f);
+            if (row < unit.rows && d < a.head_dim)
+              *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(y);
           }
-    __syncthreads();
-    const int slot = 2 * blockIdx.x + segment.slot();
-    for (int i = threadIdx.x; i < unit.rows * a.head_dim; i += kThreads) {
-      const int r = i / a.head_dim, d = i - r * a.head_dim;
-      float top = -INFINITY;
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) top = fmaxf(top, merge_m[x][r]);
-      const float base_m = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f, out = 0.0f;
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) {
-        const float f = paged_exp2(merge_m[x][r] - base_m);
-        sum = fmaf(f, merge_l[x][r], sum);
-        out = fmaf(f, reinterpret_cast<const float*>(rings + x * S::kRingBytes)[r * S::kPitch + d],
-                   out);
       }
-      if (segment.whole()) {
-        st_out(static_cast<T*>(a.out) +
-                   (static_cast<int64_t>(sequence) * a.heads + unit.first_head + r) * a.head_dim + d,
-               length == 0 ? 0.0f : out / sum);
+    } else {
+      // A part: to the ring, which is empty, when the warp is done, else out of
+      // its way.
+      const int kind = begin == 0 ? kTail : kHead;
+      const bool spilled = to_read > 0;
+      float* const part = spilled ? a.spill + range * a.row_cap * a.head_dim
+                                  : reinterpret_cast<float*>(ring);
+      const int pitch = spilled ? a.head_dim : S::kPitch;
+      if constexpr (!kTma) copy_wait<0>();
+      __syncwarp();  // every lane has read its last stage
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        const int row = g + 8 * h;
+        if (row >= unit.rows) continue;
+        if (t == 0) {
+          parts.m[warp][kind][row] = m[h];
+          parts.l[warp][kind][row] = l[h];
+        }
+#pragma unroll
+        for (int c = 0; c < kDim / 64; ++c)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+              const int d = 64 * c + 8 * (2 * t + x) + e;
+              if (d < a.head_dim)
+                *reinterpret_cast<float4*>(part + row * pitch + d) =
+                    make_float4(o[8 * c + e][2 * h + x], o[8 * c + e + 1][2 * h + x],
+                                o[8 * c + e + 2][2 * h + x], o[8 * c + e + 3][2 * h + x]);
+            }
+      }
+      if (lane == 0)
+        parts.records[warp][kind] = PartRecord{out.sequence, out.unit,     out.tiles, begin,
+                                               out.tile + 1, opens && kind == kHead, spilled};
+    }
+    if (to_read > 0) {
+      advance(out);
+      begin = 0;
+      clear();
+      if constexpr (kQueryAhead) {
+#pragma unroll
+        for (int j = 0; j < kDim / 32; ++j)
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) qa[j][h] = q_next[j][h];
+        load_next_query();
       } else {
-        const int64_t row = static_cast<int64_t>(slot) * row_cap + r;
-        a.partial[row * a.head_dim + d] = out;
-        if (d == 0) a.partial_ml[row] = make_float2(top, sum);
+        load_query(qa, out.sequence, out.unit);
       }
     }
-    // The rings go back to the TMA unit.
-    if constexpr (kTma) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
   }
   if (reported != 0) watchdog_trip(a.watchdog, reported);
+  __syncthreads();
+  paged_merge<T, kWarps, kRows, S::kRingBytes / 4, S::kPitch, 4>(
+      a, parts, reinterpret_cast<const float*>(rings));
 }
 
 // Encodes a cache for the TMA unit; false when its layout does not allow it.
@@ -535,14 +612,10 @@ bool cache_map(CUtensorMap* map, const PagedArgs& a, const void* base, int64_t p
 template <typename T, int kDim, int kRows, bool kTma, int kWarps, int kStages>
 int launch_mma(PagedArgs a, const CUtensorMap& k_map, const CUtensorMap& v_map,
                const MapOrder& order, cudaStream_t stream) {
-  constexpr int kLeast = kWarps;
-  constexpr auto kernel = paged_mma_kernel<T, kDim, kRows, kTma, kWarps, kStages, kLeast>;
+  constexpr auto kernel = paged_mma_kernel<T, kDim, kRows, kTma, kWarps, kStages>;
   constexpr size_t kShared = Shape<T, kDim, kRows, kWarps, kStages>::kShared;
-  a.parts = (a.group + kRows - 1) / kRows;
-  const int row_cap = a.group < kRows ? a.group : kRows;
-  const int grid = paged_grid(a, sm_count(), kTile, kLeast, kRows);
-  a.partial_ml = reinterpret_cast<float2*>(a.partial + static_cast<int64_t>(grid) * 2 * row_cap *
-                                                           a.head_dim);
+  const int grid = paged_grid(a, sm_count(), kTile, kWarps, kRows);
+  paged_scratch(&a, grid, kWarps, kRows);
   cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            static_cast<int>(kShared));
   if (error != cudaSuccess) return error;
@@ -556,9 +629,9 @@ int launch_mma(PagedArgs a, const CUtensorMap& k_map, const CUtensorMap& v_map,
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
-  error = cudaLaunchKernelEx(&config, kernel, a, k_map, v_map, order, row_cap);
+  error = cudaLaunchKernelEx(&config, kernel, a, k_map, v_map, order);
   if (error == cudaSuccess && grid > 1)
-    error = launch_join<T, kTile, kLeast, kRows>(a, grid, row_cap, stream);
+    error = launch_join<T, kTile, kWarps, kRows>(a, grid, stream);
   return error != cudaSuccess ? error : cudaGetLastError();
 }
 

@@ -1,16 +1,20 @@
-// How the keys of a ragged batch are cut over the CTAs of one launch, in plain
-// C++ so that it can be tested without a GPU.
+// How the keys of a ragged batch are cut over the warps and CTAs of one launch,
+// in plain C++ so that it can be tested without a GPU.
 //
 // A unit is one sequence's keys for one group of query rows (a key-value head,
 // or a part of its query heads).  Its keys are cut into tiles (an empty
 // sequence counts one); the tiles of all units are laid end to end, sequence
-// after sequence, and CTA c takes [begin(c), begin(c + 1)) of them.  Lengths
-// stay on the device, so every CTA computes the total and its own start.
+// after sequence, and every warp takes an equal range of them, the warps of a
+// CTA next to one another.  Lengths stay on the device, so every CTA computes
+// the total and where its warps start.
 //
-// A CTA's range cuts at most two units: the one it starts inside of (partial
-// slot 0) and the one it ends inside of (slot 1; when both are the same unit,
-// slot 0).  So the parts of a cut unit are slot 1 of the CTA that starts it
-// and slot 0 of the CTAs that follow, in key order.
+// A warp writes the units that it covers whole to the output.  Of the at most
+// two that its range cuts it leaves parts: its head (a unit that an earlier
+// warp starts) and its tail (a unit that it starts and does not end).  The CTA
+// joins the parts of a unit that follow one another, and a unit that reaches
+// past the CTA is left as a part of the CTA: slot 0 if an earlier CTA starts
+// it, else slot 1.  So the parts of a unit cut between CTAs are slot 1 of the
+// CTA that starts it and slot 0 of the CTAs that follow, in key order.
 #pragma once
 
 #include <cstdint>
@@ -21,41 +25,82 @@ namespace opl {
 
 OPL_HD int key_tiles(int length, int tile) { return length <= tile ? 1 : (length - 1) / tile + 1; }
 
-// CTAs that take part: each gets at least `least` tiles, but for the last
-// ones of a small call.
-OPL_HD int active_ctas(int64_t total, int ctas, int least) {
-  const int64_t useful = (total + least - 1) / least;
+// CTAs that take part: no more than give every warp a tile.
+OPL_HD int active_ctas(int64_t total, int ctas, int warps) {
+  const int64_t useful = (total + warps - 1) / warps;
   return useful < ctas ? static_cast<int>(useful) : ctas;
 }
 
-OPL_HD int64_t range_begin(int64_t total, int ctas, int cta) { return total * cta / ctas; }
+// `total` tiles over `count` ranges that differ by at most one tile, the longer
+// ones first.
+struct Ranges {
+  int64_t each;  // tiles of a shorter range
+  int64_t more;  // ranges with one tile more
 
-// The CTA whose range holds tile w.
-OPL_HD int range_owner(int64_t total, int ctas, int64_t w) {
-  return static_cast<int>(((w + 1) * ctas + total - 1) / total) - 1;
-}
-
-// One run of tiles of one unit.  `before` is the number of tiles of a single
-// unit in the sequences before `sequence`, whose units start at
-// units * before.
-struct Segment {
-  int unit;   // of the sequence, 0 .. units - 1
-  int tiles;  // of the unit
-  int begin, end;
-
-  OPL_HD bool whole() const { return begin == 0 && end == tiles; }
-  OPL_HD int slot() const { return begin == 0 ? 1 : 0; }
+  OPL_HD int64_t begin(int64_t index) const {
+    return each * index + (index < more ? index : more);
+  }
+  OPL_HD int64_t holder(int64_t tile) const {  // the range of a tile
+    const int64_t longer = (each + 1) * more;
+    return tile < longer ? tile / (each + 1) : more + (tile - longer) / each;
+  }
 };
 
-OPL_HD Segment segment_at(int64_t w, int64_t limit, int64_t before, int tiles, int units) {
-  Segment s;
+OPL_HD Ranges make_ranges(int64_t total, int count) {
+  Ranges r;
+  // 64-bit divisions take hundreds of cycles at the start of every CTA.
+  r.each = total >> 32 == 0 ? static_cast<int64_t>(static_cast<uint32_t>(total) /
+                                                   static_cast<uint32_t>(count))
+                            : total / count;
+  r.more = total - r.each * count;
+  return r;
+}
+
+// A tile of the batch: of unit `unit` (0 .. units - 1) of a sequence whose
+// units have `tiles` tiles.
+struct TilePlace {
+  int unit, tile;
+};
+
+// Place of tile `w` in the sequence that holds it; `before` is the number of
+// tiles of a single unit in the sequences before, whose units start at
+// units * before.
+OPL_HD TilePlace place_of(int64_t w, int64_t before, int tiles, int units) {
   const int64_t local = w - before * units;
-  s.tiles = tiles;
-  s.unit = static_cast<int>(local / tiles);
-  s.begin = static_cast<int>(local - static_cast<int64_t>(s.unit) * tiles);
-  const int64_t left = limit - w;
-  s.end = tiles - s.begin <= left ? tiles : static_cast<int>(s.begin + left);
-  return s;
+  TilePlace p;
+  if (local >> 32 == 0) {
+    p.unit = static_cast<int>(static_cast<uint32_t>(local) / static_cast<uint32_t>(tiles));
+  } else {
+    p.unit = static_cast<int>(local / tiles);
+  }
+  p.tile = static_cast<int>(local - static_cast<int64_t>(p.unit) * tiles);
+  return p;
+}
+
+// A part that a warp leaves, empty when begin == end.
+struct PartRecord {
+  int sequence, unit, tiles, begin, end;
+  int opens;    // a head with which the CTA's range begins
+  int spilled;  // lies in global memory, the warp's ring had more to do
+
+  OPL_HD bool empty() const { return begin == end; }
+};
+
+constexpr int kHead = 0, kTail = 1;
+
+// The parts of a CTA in key order are its warps' heads and tails, warp after
+// warp: bit 2 * warp + kind of these masks.  `present` are the parts that are
+// not empty, `starts` the first of each unit (a tail, or the head with which
+// the CTA's range begins).  The parts from a start up to the next one are one
+// unit's.
+OPL_HD bool starts_unit(const PartRecord& r, int kind) {
+  return !r.empty() && (kind == kTail || r.opens != 0);
+}
+
+OPL_HD uint32_t parts_of_unit(uint32_t present, uint32_t starts, int start) {
+  const uint32_t later = starts & ~((2u << start) - 1);
+  const uint32_t end = later & (0u - later);  // lowest; none: 0
+  return present & (end - 1) & ~((1u << start) - 1);
 }
 
 }  // namespace opl

@@ -51,64 +51,110 @@ void check_guards() {
   require(opl::readable_length(INT32_MAX, 1 << 20, 1 << 20) == INT32_MAX, "capacity past 32 bits");
 }
 
-// Every tile of every unit is taken once; whole units have no part; the parts
-// of a cut unit are where the join looks for them.
-void check_split(const std::vector<int>& lengths, int units, int tile, int grid, int least) {
+// Every tile of every unit is taken once; a unit is written by the warp that
+// takes it whole, by the CTA that joins all of its parts, or from the CTAs'
+// partial slots, which lie where the join looks for them.
+void check_split(const std::vector<int>& lengths, int units, int tile, int grid, int warps) {
   std::vector<int64_t> before(lengths.size() + 1, 0);
   for (size_t b = 0; b < lengths.size(); ++b)
     before[b + 1] = before[b] + opl::key_tiles(lengths[b], tile);
   const int64_t total = before.back() * units;
-  const int ctas = opl::active_ctas(total, grid, least);
+  const int ctas = opl::active_ctas(total, grid, warps);
   require(ctas >= 1 && ctas <= grid, "active CTAs");
+  std::vector<char> written(lengths.size() * units, 0);
   std::vector<std::vector<char>> taken(lengths.size() * units);
   for (size_t b = 0; b < lengths.size(); ++b)
     for (int u = 0; u < units; ++u)
       taken[b * units + u].assign(opl::key_tiles(lengths[b], tile), 0);
-  // Unit and first tile of each partial slot, as the CTAs fill them.
+  // Unit and tiles of each partial slot, as the CTAs fill them.
   std::vector<int64_t> slot_unit(2 * ctas, -1);
   std::vector<int> slot_begin(2 * ctas, -1), slot_end(2 * ctas, -1);
-  require(opl::range_begin(total, ctas, 0) == 0 && opl::range_begin(total, ctas, ctas) == total,
-          "ranges cover all tiles");
+  const opl::Ranges ranges = opl::make_ranges(total, ctas * warps);
+  const auto cta_start = [&](int64_t c) { return ranges.begin(c * warps); };
+  require(cta_start(0) == 0 && cta_start(ctas) == total, "ranges cover all tiles");
   for (int c = 0; c < ctas; ++c) {
-    int64_t w = opl::range_begin(total, ctas, c);
-    const int64_t limit = opl::range_begin(total, ctas, c + 1);
-    require(w < limit, "no empty range");
-    size_t b = 0;
-    while (w < limit) {
-      while (w >= before[b + 1] * units) ++b;
-      require(opl::range_owner(total, ctas, w) == c, "owner");
-      const int tiles = opl::key_tiles(lengths[b], tile);
-      const opl::Segment s = opl::segment_at(w, limit, before[b], tiles, units);
-      require(s.unit >= 0 && s.unit < units && s.begin < s.end && s.end <= tiles, "segment");
-      auto& mine = taken[b * units + s.unit];
-      for (int t = s.begin; t < s.end; ++t) {
-        require(mine[t] == 0, "a tile taken twice");
-        mine[t] = 1;
+    const int64_t cta_begin = cta_start(c);
+    require(cta_begin < cta_start(c + 1), "no empty CTA");
+    std::vector<opl::PartRecord> storage(2 * warps, opl::PartRecord{});
+    auto records = reinterpret_cast<opl::PartRecord(*)[2]>(storage.data());
+    for (int x = 0; x < warps; ++x) {
+      int64_t w = ranges.begin(static_cast<int64_t>(c) * warps + x);
+      const int64_t limit = ranges.begin(static_cast<int64_t>(c) * warps + x + 1);
+      const bool opens = w == cta_begin;
+      size_t b = 0;
+      while (w < limit) {
+        while (w >= before[b + 1] * units) ++b;
+        require(ranges.holder(w) == static_cast<int64_t>(c) * warps + x, "holder");
+        const int tiles = opl::key_tiles(lengths[b], tile);
+        const opl::TilePlace p = opl::place_of(w, before[b], tiles, units);
+        require(p.unit >= 0 && p.unit < units && p.tile >= 0 && p.tile < tiles, "place");
+        const int end = tiles - p.tile <= limit - w ? tiles : p.tile + static_cast<int>(limit - w);
+        auto& mine = taken[b * units + p.unit];
+        for (int t = p.tile; t < end; ++t) {
+          require(mine[t] == 0, "a tile taken twice");
+          mine[t] = 1;
+        }
+        w += end - p.tile;
+        if (p.tile == 0 && end == tiles) {
+          ++written[b * units + p.unit];
+          continue;
+        }
+        const int kind = p.tile == 0 ? opl::kTail : opl::kHead;
+        require(records[x][kind].empty(), "a warp has one head and one tail");
+        records[x][kind] = {static_cast<int>(b), p.unit,    tiles, p.tile, end,
+                            opens && kind == opl::kHead, w < limit};
+        require(kind == opl::kHead || w == limit, "a tail ends its warp's range");
       }
-      if (!s.whole()) {
-        const int slot = 2 * c + s.slot();
-        require(slot_unit[slot] == -1, "a partial slot used twice");
-        slot_unit[slot] = static_cast<int64_t>(b) * units + s.unit;
-        slot_begin[slot] = s.begin;
-        slot_end[slot] = s.end;
-      }
-      w += s.end - s.begin;
     }
+    uint32_t present = 0, starts = 0;
+    for (int x = 0; x < 2 * warps; ++x) {
+      present |= static_cast<uint32_t>(!storage[x].empty()) << x;
+      starts |= static_cast<uint32_t>(opl::starts_unit(storage[x], x & 1)) << x;
+    }
+    uint32_t chained = 0;
+    for (int x = 0; x < 2 * warps; ++x) {
+      if ((starts >> x & 1u) == 0) continue;
+      const uint32_t mine = opl::parts_of_unit(present, starts, x);
+      require((mine & chained) == 0 && (mine >> x & 1u) != 0, "parts of a unit");
+      chained |= mine;
+      const opl::PartRecord& r = storage[x];
+      int end = r.end;
+      for (int y = x + 1; y < 2 * warps; ++y) {
+        if ((mine >> y & 1u) == 0) continue;
+        const opl::PartRecord& next = storage[y];
+        require((mine >> (y ^ 1) & 1u) == 0, "one part of a warp");
+        require(next.sequence == r.sequence && next.unit == r.unit && next.begin == end &&
+                    next.opens == 0 && (y & 1) == opl::kHead,
+                "a part out of place in the CTA");
+        end = next.end;
+      }
+      const int64_t unit = static_cast<int64_t>(r.sequence) * units + r.unit;
+      if (r.begin == 0 && end == r.tiles) {
+        ++written[unit];
+        continue;
+      }
+      const int slot = 2 * c + (r.begin == 0 ? 1 : 0);
+      require(slot_unit[slot] == -1, "a partial slot used twice");
+      slot_unit[slot] = unit;
+      slot_begin[slot] = r.begin;
+      slot_end[slot] = end;
+    }
+    require(present == chained, "a part of the CTA not joined");
   }
   for (const auto& unit : taken)
     for (char t : unit) require(t == 1, "a tile left out");
   // The join of CTA c, as paged_join_kernel finds it.
   size_t joined = 0;
   for (int c = 0; c + 1 < ctas; ++c) {
-    const int64_t limit = opl::range_begin(total, ctas, c + 1), at = limit - 1;
+    const int64_t at = cta_start(c + 1) - 1;
     size_t b = 0;
     while (at >= before[b + 1] * units) ++b;
     const int tiles = opl::key_tiles(lengths[b], tile);
-    const opl::Segment last = opl::segment_at(at, limit, before[b], tiles, units);
-    if (last.end == tiles) continue;
-    const int64_t unit_begin = at - last.begin;
-    if (unit_begin < opl::range_begin(total, ctas, c)) continue;
-    const int end_cta = opl::range_owner(total, ctas, unit_begin + tiles - 1);
+    const opl::TilePlace last = opl::place_of(at, before[b], tiles, units);
+    if (last.tile + 1 == tiles) continue;
+    const int64_t unit_begin = at - last.tile;
+    if (unit_begin < cta_start(c)) continue;
+    const int end_cta = static_cast<int>(ranges.holder(unit_begin + tiles - 1) / warps);
     const int64_t unit = static_cast<int64_t>(b) * units + last.unit;
     int next = 0;
     for (int p = 0; p <= end_cta - c; ++p, ++joined) {
@@ -117,10 +163,12 @@ void check_split(const std::vector<int>& lengths, int units, int tile, int grid,
       next = slot_end[slot];
     }
     require(next == tiles, "a unit not joined to its end");
+    ++written[unit];
   }
   size_t parts = 0;
   for (int64_t u : slot_unit) parts += u != -1;
   require(parts == joined, "a part not joined");
+  for (char n : written) require(n == 1, "every unit is written once");
 }
 
 }  // namespace
@@ -129,16 +177,26 @@ int main() {
   check_divisions();
   check_guards();
   std::mt19937 rng(11);
+  const opl::Ranges wide = opl::make_ranges((int64_t{1} << 40) + 77, 2368);
+  for (int i = 0; i < 2368; ++i)
+    require(wide.begin(i + 1) > wide.begin(i) && wide.holder(wide.begin(i)) == i &&
+                wide.holder(wide.begin(i + 1) - 1) == i,
+            "ranges past 32 bits");
+  require(wide.begin(2368) == (int64_t{1} << 40) + 77, "ranges past 32 bits");
+  const opl::TilePlace far = opl::place_of((int64_t{1} << 36) + 5, 3, 1 << 26, 4096);
+  require(far.unit == ((int64_t{1} << 36) + 5 - 3 * 4096) >> 26 &&
+              far.tile == (((int64_t{1} << 36) + 5 - 3 * 4096) & ((1 << 26) - 1)),
+          "a place past 32 bits");
   check_split({0}, 1, 16, 296, 8);
   check_split({1}, 1, 16, 1, 8);
   check_split({131071}, 8, 16, 296, 8);
-  check_split({0, 0, 0, 5}, 3, 8, 4, 1);
-  for (int trial = 0; trial < 600; ++trial) {
-    const int batch = 1 + rng() % 40, units = 1 + rng() % 12;
-    const int most = 1 << (rng() % 12), grid = 1 + rng() % 300, least = 1 + rng() % 16;
+  check_split({0, 0, 0, 5}, 3, 8, 4, 4);
+  for (int trial = 0; trial < 3000; ++trial) {
+    const int batch = 1 + rng() % 40, units = 1 + rng() % 12, warps = 1 + rng() % 8;
+    const int most = 1 << (rng() % 12), grid = 1 + rng() % 300;
     std::vector<int> lengths(batch);
     for (int& n : lengths) n = rng() % 5 == 0 ? 0 : static_cast<int>(rng() % (most + 1));
-    check_split(lengths, units, rng() % 2 ? 8 : 16, grid, least);
+    check_split(lengths, units, rng() % 2 ? 8 : 16, grid, warps);
   }
   std::printf("PASS\n");
   return 0;
