@@ -220,7 +220,7 @@ int opl_kv_append_bf16(const opl_bf16_t* q, int64_t q_token, int64_t q_head, con
  * FP32; the result is rounded once to the tensors' type.  A sequence of length
  * 0 gives zeros.  Table entries past a sequence's pages are not read, and
  * neither are a page's tokens past its length.  Keys of a page outside the
- * cache are left out.
+ * cache are left out.  batch * max_pages * page_size is at most 2^34.
  * `workspace` is 16-byte aligned device memory of at least the size that
  * opl_paged_attention_workspace gives; its contents do not matter and need not
  * be kept, but two calls that may overlap on the GPU need one each. */

@@ -119,7 +119,6 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
   __shared__ float weights[kWarps][kRows][kTile];
   __shared__ float rescale[kWarps][kRows];
   __shared__ PagedParts<kWarps, kRows> parts;
-  __shared__ PagedStart starts[kWarps];
   extern __shared__ __align__(16) float rows[];  // [kWarps][kRows][kWidth]
   pdl_begin();
 
@@ -129,19 +128,19 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
   const T* values = static_cast<const T*>(a.v);
   const int page_size = static_cast<int>(a.page_size.divisor);
   if (lane < 2) parts.records[warp][lane] = PartRecord{};
-  const PagedTotal total = paged_start<kThreads, kTile, kWarps>(
-      a, gridDim.x, starts, [](const PagedTotal& x, int target) -> long long {
-        return static_cast<int>(blockIdx.x) < x.ctas
-                   ? x.ranges.begin(int64_t{kWarps} * blockIdx.x + target)
-                   : -1;
+  const int64_t range = int64_t{kWarps} * blockIdx.x + warp;
+  PagedStart start = {};
+  const PagedTotal total = paged_start<kTile, kWarps>(
+      a, gridDim.x, &start, [range](const PagedTotal& x) -> int64_t {
+        const int64_t at = x.ranges.begin(range);
+        return static_cast<int>(blockIdx.x) < x.ctas && at < x.tiles ? at : -1;
       });
   if (static_cast<int>(blockIdx.x) >= total.ctas) return;
-  const int64_t range = int64_t{kWarps} * blockIdx.x + warp;
   int64_t w = total.ranges.begin(range);
   const int64_t limit = total.ranges.begin(range + 1);
   const bool opens = w == total.ranges.begin(int64_t{kWarps} * blockIdx.x);
-  int sequence = starts[warp].sequence;
-  int64_t before = starts[warp].before;
+  int sequence = start.sequence;
+  int64_t before = start.before;
   int reported = 0;
 
   // Which row's score this lane holds after transpose_sum: the value index is
@@ -361,7 +360,8 @@ int paged_attention(const void* q, int64_t q_batch, int64_t q_head, const opl_kv
       batch <= 0 || heads <= 0 || max_pages <= 0 || cache->pages <= 0 || cache->page_size <= 0 ||
       cache->kv_heads <= 0 || heads % cache->kv_heads != 0 || cache->head_dim <= 0 ||
       cache->head_dim > kPagedMaxHeadDim || !(scale - scale == 0.0f) ||
-      reinterpret_cast<std::uintptr_t>(workspace) % 16 != 0)
+      reinterpret_cast<std::uintptr_t>(workspace) % 16 != 0 ||
+      static_cast<int64_t>(max_pages) * cache->page_size > kPagedMaxKeys / batch)
     return cudaErrorInvalidValue;
   size_t needed = 0;
   const int status = opl_paged_attention_workspace(heads, cache->kv_heads, cache->head_dim, &needed);

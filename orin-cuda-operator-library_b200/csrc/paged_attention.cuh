@@ -54,79 +54,74 @@ __device__ __forceinline__ int paged_length(const PagedArgs& a, int sequence) {
                          static_cast<int>(a.page_size.divisor));
 }
 
-// Where a search for a tile ended.
-struct PagedStart {
-  int64_t before;  // see place_of
-  int sequence;
-};
-
 struct PagedTotal {
   int64_t tiles;  // of all units
   int ctas;       // that take part
   Ranges ranges;  // of their warps
 };
 
-// The whole CTA (kThreads threads) adds up the sequences' tiles and finds the
-// sequences of kTargets tiles: target x is the tile place(total, x), or none
-// when that is negative.  kUnitWarps: warps of a CTA of the main launch.
-template <int kThreads, int kTile, int kUnitWarps, int kTargets, typename Place>
-__device__ __forceinline__ PagedTotal paged_start(const PagedArgs& a, int grid_ctas,
-                                                  PagedStart (&found)[kTargets], Place place) {
-  constexpr int kWarpCount = kThreads / 32;
-  static_assert(kTargets <= kThreads, "a thread for each target");
-  __shared__ long long warp_total[kWarpCount];
-  __shared__ long long wanted[kTargets];
-  const int tid = threadIdx.x;
-  const int per = (a.batch + kThreads - 1) / kThreads;
-  const int first = min(tid * per, a.batch), last = min(first + per, a.batch);
-  long long mine = 0;
-  for (int b = first; b < last; ++b) mine += key_tiles(paged_length(a, b), kTile);
-  long long running = mine;
+// The sequence of a tile.
+struct PagedStart {
+  int sequence, length, raw_length;  // as read, and as given
+  int64_t before;                    // see place_of
+};
+
+__device__ __forceinline__ uint32_t warp_prefix(uint32_t x, int lane) {  // with x itself
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long other = __shfl_up_sync(kFullMask, running, o);
-    if ((tid & 31) >= o) running += other;
+    const uint32_t other = __shfl_up_sync(kFullMask, x, o);
+    if (lane >= o) x += other;
   }
-  if ((tid & 31) == 31) warp_total[tid >> 5] = running;
-  __syncthreads();
-  long long before = running - mine, all = 0;
-#pragma unroll
-  for (int w = 0; w < kWarpCount; ++w) {
-    if (w < (tid >> 5)) before += warp_total[w];
-    all += warp_total[w];
+  return x;
+}
+
+// A warp adds up the sequences' tiles and finds the sequence of the tile
+// place(total) (none when that is negative).  Every warp does it for itself:
+// this is the start of the launch, where a barrier and what it orders would
+// cost more than the repeated loads.  kUnitWarps: warps of a CTA of the main
+// launch.  The sums fit 32 bits (see the limit on the cache's capacity).
+template <int kTile, int kUnitWarps, typename Place>
+__device__ __forceinline__ PagedTotal paged_start(const PagedArgs& a, int grid_ctas,
+                                                  PagedStart* start, Place place) {
+  const int lane = threadIdx.x & 31;
+  const int per = (a.batch + 31) / 32;
+  uint32_t mine = 0;
+#pragma unroll 4
+  for (int i = 0; i < per; ++i) {
+    const int b = lane * per + i;
+    if (b < a.batch) mine += key_tiles(paged_length(a, b), kTile);
   }
+  const uint32_t end = warp_prefix(mine, lane);
   PagedTotal total;
-  total.tiles = all * a.units.divisor;
+  total.tiles = static_cast<int64_t>(__shfl_sync(kFullMask, end, 31)) * a.units.divisor;
   total.ctas = active_ctas(total.tiles, grid_ctas, kUnitWarps);  // a tile for each warp
   total.ranges = make_ranges(total.tiles, kUnitWarps * total.ctas);
-  if (tid < kTargets) {
-    const long long at = place(total, tid);
-    wanted[tid] = at < 0 || at >= total.tiles ? -1
-                  : at >> 31 == 0             ? fast_div(static_cast<uint32_t>(at), a.units)
-                                              : at / a.units.divisor;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int x = 0; x < kTargets; ++x) {
-    const long long to = wanted[x];
-    if (to < before || to >= before + mine) continue;
-    if (per == 1) {
-      found[x].sequence = tid;
-      found[x].before = before;
-      continue;
+  const int64_t at = place(total);
+  if (at < 0) return total;
+  const uint32_t wanted =
+      at >> 31 == 0 ? fast_div(static_cast<uint32_t>(at), a.units)
+                    : static_cast<uint32_t>(at / a.units.divisor);
+  // The lane whose sequences hold it, then the sequence among them.
+  const int owner = __popc(__ballot_sync(kFullMask, end <= wanted));
+  uint32_t before = __shfl_sync(kFullMask, end - mine, owner);
+  for (int i = 0; i < per; i += 32) {
+    const int b = owner * per + i + lane;
+    const bool there = i + lane < per && b < a.batch;
+    const int raw = there ? ld_int(a.seq_lens + b) : 0;
+    const int length = readable_length(raw, a.max_pages, static_cast<int>(a.page_size.divisor));
+    const uint32_t tiles = there ? key_tiles(length, kTile) : 0;
+    const uint32_t upto = before + warp_prefix(tiles, lane);
+    const uint32_t passed = __ballot_sync(kFullMask, upto <= wanted);
+    if (passed != kFullMask) {
+      const int which = __popc(passed);
+      start->sequence = owner * per + i + which;
+      start->length = __shfl_sync(kFullMask, length, which);
+      start->raw_length = __shfl_sync(kFullMask, raw, which);
+      start->before = __shfl_sync(kFullMask, upto - tiles, which);
+      break;
     }
-    long long p = before;
-    for (int b = first; b < last; ++b) {
-      const int tiles = key_tiles(paged_length(a, b), kTile);
-      if (to < p + tiles) {
-        found[x].sequence = b;
-        found[x].before = p;
-        break;
-      }
-      p += tiles;
-    }
+    before = __shfl_sync(kFullMask, upto, 31);
   }
-  __syncthreads();
   return total;
 }
 
@@ -166,14 +161,25 @@ __device__ __forceinline__ void st_row(T* p, const float (&x)[kWidth]) {
   }
 }
 
+// kWidth consecutive floats of shared or global memory, written by this CTA.
 template <int kWidth>
-__device__ __forceinline__ void ld_row(const float* p, bool global, float (&x)[kWidth]) {
+__device__ __forceinline__ void ld_row(const float* p, float (&x)[kWidth]) {
   if constexpr (kWidth == 4) {
-    const float4 v = global ? __ldcg(reinterpret_cast<const float4*>(p))
-                            : *reinterpret_cast<const float4*>(p);
+    const float4 v = *reinterpret_cast<const float4*>(p);
     x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
   } else {
-    x[0] = global ? __ldcg(p) : *p;
+    x[0] = *p;
+  }
+}
+
+// The same written by another launch.
+template <int kWidth>
+__device__ __forceinline__ void ld_row_l2(const float* p, float (&x)[kWidth]) {
+  if constexpr (kWidth == 4) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    x[0] = __ldcg(p);
   }
 }
 
@@ -216,40 +222,34 @@ __device__ __forceinline__ void paged_merge(const PagedArgs& a, const PagedParts
     for (int i = together ? threadIdx.x : lane; i < unit.rows * pieces;
          i += together ? 32 * kWarps : 32) {
       const int row = i / pieces, d = (i - row * pieces) * kWidth;
-      // A warp has one part of a unit: the loads do not wait for one another.
-      float m[kWarps], l[kWarps], v[kWarps][kWidth];
-#pragma unroll
+      // A warp has at most one part of a unit.
+      float top = -INFINITY;
+#pragma unroll 4
       for (int b = 0; b < kWarps; ++b) {
-        m[b] = -INFINITY, l[b] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < kWidth; ++e) v[b][e] = 0.0f;
         const uint32_t kinds = mine >> (2 * b) & 3u;
-        if (kinds == 0) continue;
-        const int kind = kinds == 1u << kTail ? kTail : kHead;
-        m[b] = parts.m[b][kind][row];
-        l[b] = parts.l[b][kind][row];
-        if (parts.records[b][kind].spilled == 0)
-          ld_row(rows + b * kStride + row * kPitch + d, false, v[b]);
-        else
-          ld_row(a.spill + ((static_cast<int64_t>(blockIdx.x) * kWarps + b) * a.row_cap + row) *
-                               a.head_dim + d,
-                 true, v[b]);
+        if (kinds != 0) top = fmaxf(top, parts.m[b][kinds >> 1][row]);
       }
-      float top = m[0];
-#pragma unroll
-      for (int b = 1; b < kWarps; ++b) top = fmaxf(top, m[b]);
       const float base = top == -INFINITY ? 0.0f : top;
       float sum = 0.0f, out[kWidth] = {};
-#pragma unroll
+#pragma unroll 4
       for (int b = 0; b < kWarps; ++b) {
-        const float f = paged_exp2(m[b] - base);
-        sum = fmaf(f, l[b], sum);
+        const uint32_t kinds = mine >> (2 * b) & 3u;
+        if (kinds == 0) continue;
+        const int kind = kinds >> 1;
+        float v[kWidth];
+        ld_row(parts.records[b][kind].spilled == 0
+                   ? rows + b * kStride + row * kPitch + d
+                   : a.spill + ((static_cast<int64_t>(blockIdx.x) * kWarps + b) * a.row_cap + row) *
+                                   a.head_dim + d,
+               v);
+        const float f = paged_exp2(parts.m[b][kind][row] - base);
+        sum = fmaf(f, parts.l[b][kind][row], sum);
 #pragma unroll
-        for (int e = 0; e < kWidth; ++e) out[e] = fmaf(f, v[b][e], out[e]);
+        for (int e = 0; e < kWidth; ++e) out[e] = fmaf(f, v[e], out[e]);
       }
       if (whole) {
 #pragma unroll
-        for (int e = 0; e < kWidth; ++e) out[e] /= sum;
+        for (int e = 0; e < kWidth; ++e) out[e] = __fdividef(out[e], sum);
         st_row(static_cast<T*>(a.out) +
                    (static_cast<int64_t>(r.sequence) * a.heads + unit.first_head + row) * a.head_dim + d,
                out);
@@ -271,29 +271,32 @@ template <typename T, int kUnitTile, int kUnitWarps, int kRows, int kWidth>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a, int grid_ctas) {
   constexpr int kJoinWarps = kJoinThreads / 32;
   constexpr int kHeld = kPagedMaxHeadDim / (32 * kWidth);  // pieces of a lane
-  __shared__ PagedStart found[1];
   __shared__ float warp_top[kJoinWarps], warp_sum[kJoinWarps];
   __shared__ float rows[kJoinWarps][kPagedMaxHeadDim];
-  pdl_begin();
   const int cta = blockIdx.x;
+  // The main launch waits for everything before it and only then lets this one
+  // be scheduled, and it leaves the lengths alone: they can be read while it
+  // still runs.
   const auto cta_begin = [](const PagedTotal& t, int64_t index) {
     return t.ranges.begin(kUnitWarps * index);
   };
-  const PagedTotal total = paged_start<kJoinThreads, kUnitTile, kUnitWarps>(
-      a, grid_ctas, found, [&](const PagedTotal& t, int) -> long long {
+  PagedStart start;
+  const PagedTotal total = paged_start<kUnitTile, kUnitWarps>(
+      a, grid_ctas, &start, [&](const PagedTotal& t) -> int64_t {
         return cta + 1 < t.ctas ? cta_begin(t, cta + 1) - 1 : -1;
       });
   if (cta + 1 >= total.ctas) return;
   const int64_t at = cta_begin(total, cta + 1) - 1;  // the CTA's last tile
-  const int sequence = found[0].sequence;
-  const int tiles = key_tiles(paged_length(a, sequence), kUnitTile);
-  const TilePlace last = place_of(at, found[0].before, tiles, a.units.divisor);
+  const int sequence = start.sequence;
+  const int tiles = key_tiles(start.length, kUnitTile);
+  const TilePlace last = place_of(at, start.before, tiles, a.units.divisor);
   if (last.tile + 1 == tiles) return;  // not cut here
   const int64_t unit_begin = at - last.tile;
   if (unit_begin < cta_begin(total, cta)) return;  // an earlier CTA starts it
   const PagedUnit unit = paged_unit<kRows>(a, last.unit);
   const int row = blockIdx.y;
   if (row >= unit.rows) return;
+  pdl_begin();  // the main launch's parts
   const int parts =
       static_cast<int>(total.ranges.holder(unit_begin + tiles - 1) / kUnitWarps) - cta + 1;
   const auto part_row = [&](int p) {
@@ -321,7 +324,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
       const int d = (32 * i + lane) * kWidth;
       if (d >= a.head_dim) continue;
       float v[kWidth];
-      ld_row(a.partial + part_row(p) * a.head_dim + d, true, v);
+      ld_row_l2(a.partial + part_row(p) * a.head_dim + d, v);
 #pragma unroll
       for (int e = 0; e < kWidth; ++e) out[i][e] = fmaf(f, v[e], out[i][e]);
     }
@@ -338,7 +341,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
     for (int w = 0; w < kJoinWarps; ++w) l += warp_sum[w], o += rows[w][d];
     st_out(static_cast<T*>(a.out) +
                (static_cast<int64_t>(sequence) * a.heads + unit.first_head + row) * a.head_dim + d,
-           o / l);
+           __fdividef(o, l));
   }
 }
 
@@ -351,6 +354,10 @@ cudaError_t launch_join(const PagedArgs& a, int grid_ctas, cudaStream_t stream) 
   return launch_pdl(paged_join_kernel<T, kUnitTile, kUnitWarps, kRows, 1>, grid, block, stream, a,
                     grid_ctas);
 }
+
+// Keys that a block table may have room for, all sequences together: the
+// schedule counts tiles of 8 keys and more in 32 bits.
+constexpr int64_t kPagedMaxKeys = int64_t{1} << 34;
 
 // The most CTAs of a launch; the workspace is sized for them.
 inline int paged_grid_limit() { return 2 * sm_count(); }

@@ -146,7 +146,6 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   constexpr int kHalves = kRows / 8;  // row groups of the S accumulator in use
   extern __shared__ unsigned char shared[];
   __shared__ PagedParts<kWarps, kRows> parts;
-  __shared__ PagedStart starts[kWarps];
   __shared__ uint64_t full[kWarps][kStages];
   __shared__ int abort_wait;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -166,21 +165,20 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       }
     }
   }
+  __syncthreads();
   pdl_begin();
 
   const T* q = static_cast<const T*>(a.q);
   const int page_size = static_cast<int>(a.page_size.divisor);
   if (lane < 2) parts.records[warp][lane] = PartRecord{};
-  // The barriers are also set up before the first copy by this search's
-  // __syncthreads.
-  const PagedTotal total = paged_start<kThreads, kTile, kWarps>(
-      a, gridDim.x, starts, [](const PagedTotal& x, int target) -> long long {
-        return static_cast<int>(blockIdx.x) < x.ctas
-                   ? x.ranges.begin(int64_t{kWarps} * blockIdx.x + target)
-                   : -1;
+  const int64_t range = int64_t{kWarps} * blockIdx.x + warp;
+  PagedStart start;
+  const PagedTotal total = paged_start<kTile, kWarps>(
+      a, gridDim.x, &start, [range](const PagedTotal& x) -> int64_t {
+        const int64_t at = x.ranges.begin(range);
+        return static_cast<int>(blockIdx.x) < x.ctas && at < x.tiles ? at : -1;
       });
   if (static_cast<int>(blockIdx.x) >= total.ctas) return;
-  const int64_t range = int64_t{kWarps} * blockIdx.x + warp;
   const int64_t w = total.ranges.begin(range);
   const bool opens = w == total.ranges.begin(int64_t{kWarps} * blockIdx.x);
   int64_t to_fetch = total.ranges.begin(range + 1) - w, to_read = to_fetch;
@@ -219,49 +217,65 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   };
   Cursor in = {};
   if (to_read > 0) {
-    in.sequence = starts[warp].sequence;
-    enter(in, load_length(in.sequence));
-    const TilePlace p = place_of(w, starts[warp].before, in.tiles, units);
+    if (start.raw_length != start.length) reported = kBadLength;
+    in.sequence = start.sequence;
+    in.length = start.length;
+    in.tiles = key_tiles(in.length, kTile);
+    in.next_length = load_length(in.sequence + 1);
+    const TilePlace p = place_of(w, start.before, in.tiles, units);
     in.unit = p.unit;
     in.tile = p.tile;
   }
   Cursor out = in;
 
-  // The key that this lane places in a tile: with the TMA unit the first of a
-  // box of 16 or 8 (even and odd lanes: first and second half of the tile),
-  // else lanes 0-15 a key each and lanes 16-31 their values.  Its block-table
-  // entry is loaded a step before the tile is copied.
-  struct Fetched {
-    int first, length, kv_head;  // of the tile; length < 0: no tile
-    int page;                    // of this lane's key
+  // Block-table entries are loaded for a batch of tiles of one unit, a batch
+  // ahead: with the TMA unit 16 tiles of two boxes of 8 keys (one of 16: the
+  // even lanes), a lane each; else two tiles, a lane for each key.
+  constexpr int kBatch = kTma ? 16 : 2;
+  constexpr int kBatchLanes = 32 / kBatch, kKeysPerLane = kTile / kBatchLanes;
+  struct Batch {
+    int tile, left, length, kv_head;
+    int page;  // of this lane's key
   };
-  const int key_offset = kTma ? 8 * (lane & 1) : lane & 15;
   const auto fetch = [&]() {
-    Fetched f = {0, -1, 0, 0};
+    Batch f = {};
     if (to_fetch > 0) {
-      --to_fetch;
-      f.first = in.tile * kTile;
+      f.tile = in.tile;
+      f.left = min(min(kBatch, in.tiles - in.tile), static_cast<int>(min(to_fetch, int64_t{kBatch})));
       f.length = in.length;
       f.kv_head = static_cast<int>(fast_div(in.unit, a.parts));
-      const int key = f.first + key_offset;
+      const int key = (in.tile + lane / kBatchLanes) * kTile + lane % kBatchLanes * kKeysPerLane;
       if (key < in.length)
         f.page = ld_int(a.block_table + in.sequence * a.table_row + fast_div(key, a.page_size));
+      to_fetch -= f.left;
+      in.tile += f.left - 1;
       advance(in);
     }
     return f;
   };
   // Copies a tile into the next stage; bit j of the result: key j is there.
-  const auto issue = [&](const Fetched& f) -> uint32_t {
+  Batch batch = {}, next_batch = {};
+  int batch_lane = 0;
+  const auto issue = [&]() -> uint32_t {
     uint32_t there = 0;
-    if (f.length >= 0) {
-      const int key = f.first + key_offset;
-      const bool known = key < f.length;
-      const bool ok = known && cache_page(f.page, a.pages);
+    while (batch.left == 0 && (next_batch.left > 0 || to_fetch > 0)) {
+      batch = next_batch;
+      batch_lane = lane % kBatchLanes;
+      next_batch = fetch();
+    }
+    if (batch.left > 0) {
+      const int page = __shfl_sync(kFullMask, batch.page, batch_lane);
+      batch_lane += kBatchLanes;
+      --batch.left;
+      const int first = batch.tile++ * kTile;
+      const int key = first + lane % kBatchLanes * kKeysPerLane;
+      const bool known = key < batch.length;
+      const bool ok = known && cache_page(page, a.pages);
       if (known && !ok) reported = kBadPage;
       const int inside = key - static_cast<int>(fast_div(key, a.page_size)) * page_size;
       if constexpr (kTma) {
         const uint32_t halves = __ballot_sync(kFullMask, ok) & 3u;
-        const int left = f.length - f.first;
+        const int left = batch.length - first;
         there = left >= kTile ? 0xffffu : (1u << left) - 1;
         if ((halves & 1u) == 0) there &= 0xff00u;
         if ((halves & 2u) == 0) there &= 0x00ffu;
@@ -270,9 +284,9 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         __syncwarp();
         if (lane < order.boxes) {
           // A box that holds no key lies past the last page: zeros.
-          const int p = ok ? f.page : static_cast<int>(a.pages);
-          const int y = order.token_first ? inside : f.kv_head;
-          const int z = order.token_first ? f.kv_head : inside;
+          const int p = ok ? page : static_cast<int>(a.pages);
+          const int y = order.token_first ? inside : batch.kv_head;
+          const int z = order.token_first ? batch.kv_head : inside;
           unsigned char* dst = ring + slot_in * S::kStageBytes + lane * 1024;
 #pragma unroll
           for (int c = 0; c < kDim / 64; ++c)
@@ -284,8 +298,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       } else {
         const int64_t place =
             !ok         ? -1
-            : lane < 16 ? f.page * a.k_page + inside * a.k_token + f.kv_head * a.k_head
-                        : f.page * a.v_page + inside * a.v_token + f.kv_head * a.v_head;
+            : lane < 16 ? page * a.k_page + inside * a.k_token + batch.kv_head * a.k_head
+                        : page * a.v_page + inside * a.v_token + batch.kv_head * a.v_head;
         there = __ballot_sync(kFullMask, ok) & 0xffffu;
         // Eight lanes copy 128 bytes of one row.
         const int piece = lane & 7;
@@ -308,17 +322,6 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     if constexpr (!kTma) copy_commit();
     return there;
   };
-
-  uint32_t there[kStages];
-  Fetched fetched;
-  {
-    Fetched early[kStages - 1];
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) early[i] = fetch();
-    fetched = fetch();
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) there[i] = issue(early[i]);
-  }
 
   // Q in the order of the key pieces: words 0, 1 of piece j are the first
   // instruction's two k pairs, words 2, 3 the second's.  The next segment's is
@@ -362,10 +365,21 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     if constexpr (kQueryAhead) load_next_query();
   }
 
+  // Step s copies tile s and, once kStages - 1 tiles are on their way, reads
+  // tile s - (kStages - 1).  (One loop for the first steps and the others:
+  // code that runs once costs its instruction fetches, about as long as the
+  // copies take.)
+  uint32_t there[kStages] = {};
+  int early = kStages - 1;
   while (to_read > 0) {
     __syncwarp();  // every lane has read the stage that is filled next
-    there[kStages - 1] = issue(fetched);
-    fetched = fetch();
+#pragma unroll
+    for (int x = 0; x + 1 < kStages; ++x) there[x] = there[x + 1];
+    there[kStages - 1] = issue();
+    if (early > 0) {
+      --early;
+      continue;
+    }
     if constexpr (kTma) {
       if (!tc::mbar_wait_warp(&full[warp][slot_out], parity, &abort_wait, a.watchdog,
                               tc::kWatchdogPaged)) {
@@ -409,8 +423,6 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         for (int x = 0; x < 2 * kHalves; ++x)
           if ((seen >> (8 * n + 2 * t + (x & 1)) & 1u) == 0) s[n][x] = -INFINITY;
     }
-#pragma unroll
-    for (int x = 0; x + 1 < kStages; ++x) there[x] = there[x + 1];
 
     float m_new[kHalves];
     bool moved = false;
@@ -504,63 +516,56 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
           if (o[n][2 + x] == o[n][2 + x]) o[n][x] += o[n][2 + x];
     }
     const PagedUnit unit = paged_unit<kRows>(a, out.unit);
+    const bool whole = begin == 0 && out.tile + 1 == out.tiles;
+    // A part goes to the ring, which is empty, when the warp is done, else out
+    // of its way.
+    const bool spilled = to_read > 0;
+    const int kind = begin == 0 ? kTail : kHead;
+    float* const part = spilled ? a.spill + range * a.row_cap * a.head_dim
+                                : reinterpret_cast<float*>(ring);
+    const int pitch = spilled ? a.head_dim : S::kPitch;
+    if constexpr (!kTma) {
+      if (!whole) copy_wait<0>();
+    }
+    __syncwarp();  // every lane has read its last stage
     // The lane's rows are g + 8h; of piece c it holds columns 8 (2t + x) + e in
     // o[8c + e][2h + x].
-    if (begin == 0 && out.tile + 1 == out.tiles) {
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const int row = g + 8 * h;
-        const float f = out.length == 0 ? 0.0f : 1.0f / l[h];
-        T* const dst =
-            static_cast<T*>(a.out) +
-            (static_cast<int64_t>(out.sequence) * a.heads + unit.first_head + row) * a.head_dim;
+    for (int h = 0; h < kHalves; ++h) {
+      const int row = g + 8 * h;
+      if (row >= unit.rows) continue;
+      T* const dst =
+          static_cast<T*>(a.out) +
+          (static_cast<int64_t>(out.sequence) * a.heads + unit.first_head + row) * a.head_dim;
+      const float f = !whole ? 1.0f : out.length == 0 ? 0.0f : __fdividef(1.0f, l[h]);
 #pragma unroll
-        for (int c = 0; c < kDim / 64; ++c)
+      for (int c = 0; c < kDim / 64; ++c)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int d = 64 * c + 8 * (2 * t + x);
-            alignas(16) T y[8];
+        for (int x = 0; x < 2; ++x) {
+          const int d = 64 * c + 8 * (2 * t + x);
+          if (d >= a.head_dim) continue;
+          float y[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) st_out(&y[e], o[8 * c + e][2 * h + x] * f);
-            if (row < unit.rows && d < a.head_dim)
-              *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(y);
+          for (int e = 0; e < 8; ++e) y[e] = o[8 * c + e][2 * h + x] * f;
+          if (whole) {
+            alignas(16) T z[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) st_out(&z[e], y[e]);
+            *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(z);
+          } else {
+            float4* const to = reinterpret_cast<float4*>(part + row * pitch + d);
+            to[0] = make_float4(y[0], y[1], y[2], y[3]);
+            to[1] = make_float4(y[4], y[5], y[6], y[7]);
           }
-      }
-    } else {
-      // A part: to the ring, which is empty, when the warp is done, else out of
-      // its way.
-      const int kind = begin == 0 ? kTail : kHead;
-      const bool spilled = to_read > 0;
-      float* const part = spilled ? a.spill + range * a.row_cap * a.head_dim
-                                  : reinterpret_cast<float*>(ring);
-      const int pitch = spilled ? a.head_dim : S::kPitch;
-      if constexpr (!kTma) copy_wait<0>();
-      __syncwarp();  // every lane has read its last stage
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const int row = g + 8 * h;
-        if (row >= unit.rows) continue;
-        if (t == 0) {
-          parts.m[warp][kind][row] = m[h];
-          parts.l[warp][kind][row] = l[h];
         }
-#pragma unroll
-        for (int c = 0; c < kDim / 64; ++c)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-              const int d = 64 * c + 8 * (2 * t + x) + e;
-              if (d < a.head_dim)
-                *reinterpret_cast<float4*>(part + row * pitch + d) =
-                    make_float4(o[8 * c + e][2 * h + x], o[8 * c + e + 1][2 * h + x],
-                                o[8 * c + e + 2][2 * h + x], o[8 * c + e + 3][2 * h + x]);
-            }
+      if (!whole && t == 0) {
+        parts.m[warp][kind][row] = m[h];
+        parts.l[warp][kind][row] = l[h];
       }
-      if (lane == 0)
-        parts.records[warp][kind] = PartRecord{out.sequence, out.unit,     out.tiles, begin,
-                                               out.tile + 1, opens && kind == kHead, spilled};
     }
+    if (!whole && lane == 0)
+      parts.records[warp][kind] = PartRecord{out.sequence, out.unit,     out.tiles, begin,
+                                             out.tile + 1, opens && kind == kHead, spilled};
     if (to_read > 0) {
       advance(out);
       begin = 0;
