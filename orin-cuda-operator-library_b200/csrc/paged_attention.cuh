@@ -84,12 +84,27 @@ template <int kTile, int kUnitWarps, typename Place>
 __device__ __forceinline__ PagedTotal paged_start(const PagedArgs& a, int grid_ctas,
                                                   PagedStart* start, Place place) {
   const int lane = threadIdx.x & 31;
-  const int per = (a.batch + 31) / 32;
+  // Lane x adds up the tiles of `per` sequences: its own loads up to 512
+  // sequences, beyond that (1024: 68 against 74 us for the call) sums of 32 that
+  // the warp loads together.
   uint32_t mine = 0;
+  int per = (a.batch + 31) / 32;
+  if (per <= 16) {
 #pragma unroll 4
-  for (int i = 0; i < per; ++i) {
-    const int b = lane * per + i;
-    if (b < a.batch) mine += key_tiles(paged_length(a, b), kTile);
+    for (int i = 0; i < per; ++i) {
+      const int b = lane * per + i;
+      if (b < a.batch) mine += key_tiles(paged_length(a, b), kTile);
+    }
+  } else {
+    per = 32 * ((per + 31) / 32);
+    int adder = 0, left = per;
+#pragma unroll 8
+    for (int b = lane; b - lane < a.batch; b += 32) {
+      const uint32_t sum =
+          __reduce_add_sync(kFullMask, b < a.batch ? key_tiles(paged_length(a, b), kTile) : 0u);
+      if (lane == adder) mine += sum;
+      if ((left -= 32) == 0) left = per, ++adder;
+    }
   }
   const uint32_t end = warp_prefix(mine, lane);
   PagedTotal total;

@@ -37,8 +37,6 @@
 //
 // Running maximum, sum and output are FP32 in registers; the warps of a CTA
 // merge at the end of a segment, and cut units are joined by a second launch.
-#include <utility>
-
 #include "paged_attention.cuh"
 #include "tc_common.cuh"
 #include "tmap.cuh"
@@ -48,6 +46,7 @@ namespace opl {
 namespace {
 
 constexpr int kTile = 16;
+
 template <typename T>
 struct Mma;
 template <>
@@ -130,10 +129,13 @@ struct Shape {
   static_assert(kShared <= 222 * 1024, "beside the static arrays");
 };
 
-// How the tensor maps of the caches are laid out.
+// How the tensor maps of the caches are laid out: dimensions (64 columns,
+// token, 64-column piece, head, page).
 struct MapOrder {
-  int token_first;  // dimensions (head_dim, token, head, page), else head before token
-  int boxes;        // of a tile: one of 16 tokens, or two of 8
+  int boxes;   // of a tile: one of 16 tokens, or two of 8
+  int copies;  // of a box: all pieces at once, or each by itself where a box is
+               // not 16 tokens or the last piece is short (the map then has one
+               // piece, of head_dim columns)
 };
 
 // Copies are made by the TMA unit, or by the lanes (kTma false).
@@ -142,7 +144,6 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     paged_mma_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap k_map,
                      const __grid_constant__ CUtensorMap v_map, const MapOrder order) {
   using S = Shape<T, kDim, kRows, kWarps, kStages>;
-  constexpr int kThreads = 32 * kWarps;
   constexpr int kHalves = kRows / 8;  // row groups of the S accumulator in use
   extern __shared__ unsigned char shared[];
   __shared__ PagedParts<kWarps, kRows> parts;
@@ -235,7 +236,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   constexpr int kBatchLanes = 32 / kBatch, kKeysPerLane = kTile / kBatchLanes;
   struct Batch {
     int tile, left, length, kv_head;
-    int page;  // of this lane's key
+    int page, inside;  // of this lane's key; page -1: no key
+    uint32_t whole;    // bit of each lane: its keys' page is in the cache
   };
   const auto fetch = [&]() {
     Batch f = {};
@@ -245,62 +247,65 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       f.length = in.length;
       f.kv_head = static_cast<int>(fast_div(in.unit, a.parts));
       const int key = (in.tile + lane / kBatchLanes) * kTile + lane % kBatchLanes * kKeysPerLane;
-      if (key < in.length)
-        f.page = ld_int(a.block_table + in.sequence * a.table_row + fast_div(key, a.page_size));
+      const int row = static_cast<int>(fast_div(key, a.page_size));
+      f.inside = key - row * page_size;
+      f.page = -1;
+      if (key < in.length) f.page = ld_int(a.block_table + in.sequence * a.table_row + row);
       to_fetch -= f.left;
       in.tile += f.left - 1;
       advance(in);
     }
     return f;
   };
-  // Copies a tile into the next stage; bit j of the result: key j is there.
   Batch batch = {}, next_batch = {};
   int batch_lane = 0;
+  // Copies a tile into the next stage; bit j of the result: key j is there.
   const auto issue = [&]() -> uint32_t {
     uint32_t there = 0;
     while (batch.left == 0 && (next_batch.left > 0 || to_fetch > 0)) {
       batch = next_batch;
-      batch_lane = lane % kBatchLanes;
       next_batch = fetch();
+      batch_lane = lane % kBatchLanes;
+      const bool known = (batch.tile + lane / kBatchLanes) * kTile +
+                             lane % kBatchLanes * kKeysPerLane < batch.length;
+      const bool ok = cache_page(batch.page, a.pages);
+      if (known && !ok) reported = kBadPage;
+      if (!known || !ok) batch.page = -1;
+      batch.whole = __ballot_sync(kFullMask, batch.page >= 0);
     }
     if (batch.left > 0) {
       const int page = __shfl_sync(kFullMask, batch.page, batch_lane);
+      const int inside = __shfl_sync(kFullMask, batch.inside, batch_lane);
+      // The bits of this tile's lanes.
+      const uint32_t pages = batch.whole >> (batch_lane - lane % kBatchLanes);
       batch_lane += kBatchLanes;
       --batch.left;
-      const int first = batch.tile++ * kTile;
-      const int key = first + lane % kBatchLanes * kKeysPerLane;
-      const bool known = key < batch.length;
-      const bool ok = known && cache_page(page, a.pages);
-      if (known && !ok) reported = kBadPage;
-      const int inside = key - static_cast<int>(fast_div(key, a.page_size)) * page_size;
+      const int left = batch.length - batch.tile++ * kTile;
       if constexpr (kTma) {
-        const uint32_t halves = __ballot_sync(kFullMask, ok) & 3u;
-        const int left = batch.length - first;
         there = left >= kTile ? 0xffffu : (1u << left) - 1;
-        if ((halves & 1u) == 0) there &= 0xff00u;
-        if ((halves & 2u) == 0) there &= 0x00ffu;
+        if ((pages & 3u) != 3u) {
+          if ((pages & 1u) == 0) there &= 0xff00u;
+          if ((pages & 2u) == 0) there &= 0x00ffu;
+        }
         uint64_t* const bar = &full[warp][slot_in];
         if (lane == 0) tc::mbar_expect_tx(bar, S::kStageBytes);
         __syncwarp();
         if (lane < order.boxes) {
           // A box that holds no key lies past the last page: zeros.
-          const int p = ok ? page : static_cast<int>(a.pages);
-          const int y = order.token_first ? inside : batch.kv_head;
-          const int z = order.token_first ? batch.kv_head : inside;
+          const int p = page >= 0 ? page : static_cast<int>(a.pages);
           unsigned char* dst = ring + slot_in * S::kStageBytes + lane * 1024;
-#pragma unroll
-          for (int c = 0; c < kDim / 64; ++c)
-            tc::tma_load_4d(dst + c * 2048, &k_map, 64 * c, y, z, p, bar);
-#pragma unroll
-          for (int c = 0; c < kDim / 64; ++c)
-            tc::tma_load_4d(dst + S::kKeyBytes + c * 2048, &v_map, 64 * c, y, z, p, bar);
+#pragma unroll 1
+          for (int c = 0; c < order.copies; ++c, dst += 2048) {
+            tc::tma_load_5d(dst, &k_map, 64 * c, inside, 0, batch.kv_head, p, bar);
+            tc::tma_load_5d(dst + S::kKeyBytes, &v_map, 64 * c, inside, 0, batch.kv_head, p, bar);
+          }
         }
       } else {
         const int64_t place =
-            !ok         ? -1
+            page < 0    ? -1
             : lane < 16 ? page * a.k_page + inside * a.k_token + batch.kv_head * a.k_head
                         : page * a.v_page + inside * a.v_token + batch.kv_head * a.v_head;
-        there = __ballot_sync(kFullMask, ok) & 0xffffu;
+        there = pages & 0xffffu;
         // Eight lanes copy 128 bytes of one row.
         const int piece = lane & 7;
         const uint32_t dst = ring_address + slot_in * S::kStageBytes;
@@ -400,21 +405,22 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     const uint32_t stage = ring_address + slot_out * S::kStageBytes;
     if (++slot_out == kStages) slot_out = 0, parity ^= 1u;
 
-    float s[2][4] = {};
+    // Four chains of dependent instructions instead of two.
+    float s[2][4] = {}, s_odd[2][4] = {};
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int j = 0; j < kDim / 32; ++j)
 #pragma unroll
-      for (int j = 0; j < kDim / 32; ++j) {
+      for (int n = 0; n < 2; ++n) {
         const uint4 b = ld_shared(stage + (k_piece ^ (j & 1) * 16) + (j / 2) * 2048 + n * 1024);
         Mma<T>::run(s[n], qa[j][0].x, kHalves == 2 ? qa[j][kHalves - 1].x : 0u, qa[j][0].y,
                     kHalves == 2 ? qa[j][kHalves - 1].y : 0u, b.x, b.y);
-        Mma<T>::run(s[n], qa[j][0].z, kHalves == 2 ? qa[j][kHalves - 1].z : 0u, qa[j][0].w,
+        Mma<T>::run(s_odd[n], qa[j][0].z, kHalves == 2 ? qa[j][kHalves - 1].z : 0u, qa[j][0].w,
                     kHalves == 2 ? qa[j][kHalves - 1].w : 0u, b.z, b.w);
       }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int x = 0; x < 2 * kHalves; ++x) s[n][x] *= a.scale_log2;
+      for (int x = 0; x < 2 * kHalves; ++x) s[n][x] = (s[n][x] + s_odd[n][x]) * a.scale_log2;
     const uint32_t seen = there[0];
     if (seen != 0xffffu) {
 #pragma unroll
@@ -592,17 +598,15 @@ template <typename T>
 bool cache_map(CUtensorMap* map, const PagedArgs& a, const void* base, int64_t page, int64_t token,
                int64_t head, const MapOrder& order) {
   const uint64_t page_size = a.page_size.divisor;
-  uint64_t extent[4] = {static_cast<uint64_t>(a.head_dim), page_size,
-                        static_cast<uint64_t>(a.kv_heads), static_cast<uint64_t>(a.pages)};
-  int64_t stride[3] = {token, head, page};
-  uint32_t box[4] = {64, static_cast<uint32_t>(kTile / order.boxes), 1, 1};
-  if (!order.token_first) {
-    std::swap(extent[1], extent[2]);
-    std::swap(stride[0], stride[1]);
-    std::swap(box[1], box[2]);
-  }
-  uint64_t bytes[3];
-  for (int i = 0; i < 3; ++i) {
+  const uint64_t pieces = order.copies == 1 ? (a.head_dim + 63) / 64 : 1;
+  const uint64_t extent[5] = {static_cast<uint64_t>(order.copies == 1 && a.head_dim > 64 ? 64 : a.head_dim),
+                        page_size, pieces, static_cast<uint64_t>(a.kv_heads),
+                        static_cast<uint64_t>(a.pages)};
+  int64_t stride[4] = {token, 64, head, page};
+  const uint32_t box[5] = {64, static_cast<uint32_t>(kTile / order.boxes), static_cast<uint32_t>(pieces), 1,
+                     1};
+  uint64_t bytes[4];
+  for (int i = 0; i < 4; ++i) {
     // A dimension of one element may come with any stride.
     if (extent[i + 1] == 1) stride[i] = 8;
     if (stride[i] <= 0 || stride[i] >= (int64_t{1} << 39)) return false;
@@ -610,7 +614,7 @@ bool cache_map(CUtensorMap* map, const PagedArgs& a, const void* base, int64_t p
   }
   const CUtensorMapDataType type = sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-  return encode_tmap(map, type, 4, base, extent, bytes, box, CU_TENSOR_MAP_SWIZZLE_128B) ==
+  return encode_tmap(map, type, 5, base, extent, bytes, box, CU_TENSOR_MAP_SWIZZLE_128B) ==
          cudaSuccess;
 }
 
@@ -644,12 +648,12 @@ template <typename T, int kRows, bool kTma>
 int pick_dim(const PagedArgs& a, const CUtensorMap& k_map, const CUtensorMap& v_map,
              const MapOrder& order, cudaStream_t stream) {
   // About 192 KB of rings a CTA, one CTA a SM.
-  if (a.head_dim <= 64) return launch_mma<T, 64, kRows, kTma, 8, 6>(a, k_map, v_map, order, stream);
+  if (a.head_dim <= 64) return launch_mma<T, 64, kRows, kTma, 8, 3>(a, k_map, v_map, order, stream);
   if (a.head_dim <= 128)
-    return launch_mma<T, 128, kRows, kTma, 8, 3>(a, k_map, v_map, order, stream);
+    return launch_mma<T, 128, kRows, kTma, 8, 2>(a, k_map, v_map, order, stream);
   if (a.head_dim <= 192)
-    return launch_mma<T, 192, kRows, kTma, 4, 4>(a, k_map, v_map, order, stream);
-  return launch_mma<T, 256, kRows, kTma, 4, 3>(a, k_map, v_map, order, stream);
+    return launch_mma<T, 192, kRows, kTma, 4, 3>(a, k_map, v_map, order, stream);
+  return launch_mma<T, 256, kRows, kTma, 4, 2>(a, k_map, v_map, order, stream);
 }
 
 }  // namespace
@@ -658,7 +662,8 @@ template <typename T>
 int paged_attention_mma(PagedArgs a, cudaStream_t stream) {
   if (a.pages > 0x7fffffff) a.pages = 0x7fffffff;  // as far as block-table entries reach
   CUtensorMap k_map = {}, v_map = {};
-  MapOrder order = {a.k_token < a.k_head ? 1 : 0, a.page_size.divisor % kTile == 0 ? 1 : 2};
+  MapOrder order = {a.page_size.divisor % kTile == 0 ? 1 : 2, (a.head_dim + 63) / 64};
+  if (order.boxes == 1 && a.head_dim % 64 == 0) order.copies = 1;
   const bool tma =
       a.page_size.divisor % 8 == 0 &&
       cache_map<T>(&k_map, a, a.k, a.k_page, a.k_token, a.k_head, order) &&

@@ -161,10 +161,10 @@ cudaError_t encode_tmap(CUtensorMap* map, CUtensorMapDataType dtype, int rank,
       g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   });
   if (g_encode == nullptr) return cudaErrorNotSupported;
-  cuuint64_t gdim[4];
-  cuuint64_t gstride[3];
-  cuuint32_t boxdim[4];
-  cuuint32_t estride[4] = {1, 1, 1, 1};
+  cuuint64_t gdim[5];
+  cuuint64_t gstride[4];
+  cuuint32_t boxdim[5];
+  cuuint32_t estride[5] = {1, 1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) {
     gdim[i] = dims[i];
     boxdim[i] = box[i];

@@ -115,13 +115,14 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// 4-D tiled load.
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y,
-                                            int z, int w, uint64_t* bar) {
+// 5-D tiled load.
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int x, int y,
+                                            int z, int w, int v, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v),
+      "r"(smem_u32(bar))
       : "memory");
 }
 

@@ -8,7 +8,7 @@
 
 namespace opl {
 
-// Encodes a tiled tensor map of `rank` (2 to 4) dimensions.  dims[0] is the
+// Encodes a tiled tensor map of `rank` (2 to 5) dimensions.  dims[0] is the
 // innermost (contiguous) extent; strides_bytes[i] is the byte stride of
 // dimension i+1 (must be a multiple of 16).  Out-of-bounds elements read as
 // zero.  Returns cudaErrorInvalidValue when the driver rejects the map.
