@@ -5,16 +5,16 @@
 //   out[b, h] = sum_j p_j V_j,  p_j = exp(s_j - max s) / sum_i exp(s_i - max s),
 //   s_j = scale * q[b, h] . K_j,  j < seq_lens[b], keys through the block table.
 //
-// This file has the SIMT kernel, which runs FP32 caches and every 16-bit
-// cache that the tensor-core kernel does not take, the launch that joins the
-// parts of units cut between CTAs, and the entry points.
+// This file has the entry points and the kernel for what the streaming kernels
+// (paged_attention_mma.cu, paged_attention_f32.cu) do not take: rows that are no
+// multiples of 16 bytes, or lie on other boundaries.
 //
-// SIMT kernel.  The 32 lanes of a warp share a key: lane l holds E elements
-// of the queries (up to 8 rows), of the key, of the value and of the output.
-// A warp takes 8 keys at a time: E products a lane, row and key; the 8 x rows
-// sums over 32 lanes by a transposing butterfly (about one shuffle a sum
-// instead of five); one exponential a key and row; running maximum and sum
-// (log2 domain) and the output in registers.
+// The 32 lanes of a warp share a key: lane l holds elements l, l + 32, ... of
+// the queries (up to 4 rows), of the key, of the value and of the output.  A
+// warp takes 8 keys at a time; their scores are summed over the lanes by a
+// transposing butterfly (about one shuffle a sum instead of five); one
+// exponential a key and row; running maximum and sum (log2 domain) and the
+// output in registers.  Loads are of one element: their issue bounds it.
 #include "paged_attention.cuh"
 
 namespace opl {
@@ -44,50 +44,22 @@ __device__ __forceinline__ float ld_f32(const __nv_bfloat16* p) {
   return __bfloat162float(__ushort_as_bfloat16(b));
 }
 
-// Element e of a lane is element `column` of the head: vectors of up to four
-// consecutive floats when kVec, else every 32nd element.
-template <int E, bool kVec>
-__device__ __forceinline__ int column(int lane, int e) {
-  if (!kVec) return lane + 32 * e;
-  constexpr int kWidth = E < 4 ? E : 4;
-  return lane * kWidth + (e / kWidth) * 32 * kWidth + e % kWidth;
-}
+constexpr int kElements = kPagedMaxHeadDim / 32;  // of a lane
 
-// A row of a head into the lane's E registers, zero past `dim` and where the
-// row is not there.
-template <typename T, int E, bool kVec>
-__device__ __forceinline__ void load_row(const T* row, int dim, int lane, float (&x)[E]) {
-  if constexpr (kVec) {
-    constexpr int kWidth = E < 4 ? E : 4;
+// A row of a head into the lane's registers, zero past `dim` and where the row
+// is not there.
+template <typename T>
+__device__ __forceinline__ void load_row(const T* row, int dim, int lane, float (&x)[kElements]) {
 #pragma unroll
-    for (int c = 0; c < E; c += kWidth) {
-      const int d = column<E, kVec>(lane, c);
-      const bool there = row != nullptr && d < dim;
-      if constexpr (kWidth == 4) {
-        const float4 w = there ? ld_stream(reinterpret_cast<const float4*>(row + d))
-                               : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[c] = w.x, x[c + 1] = w.y, x[c + 2] = w.z, x[c + 3] = w.w;
-      } else {
-        float2 w = make_float2(0.f, 0.f);
-        if (there)
-          asm volatile("ld.global.nc.L1::no_allocate.v2.f32 {%0,%1}, [%2];"
-                       : "=f"(w.x), "=f"(w.y)
-                       : "l"(row + d));
-        x[c] = w.x, x[c + 1] = w.y;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = column<E, kVec>(lane, e);
-      x[e] = row != nullptr && d < dim ? ld_f32(row + d) : 0.0f;
-    }
+  for (int e = 0; e < kElements; ++e) {
+    const int d = lane + 32 * e;
+    x[e] = row != nullptr && d < dim ? ld_f32(row + d) : 0.0f;
   }
 }
 
-// Sums v[i] over the warp for each of kCount values (a power of two, 8 to
-// 64).  Afterwards v[0] (and v[1] for 64) of lane l is the sum of value
-// index_of(l) (+ 1).
+// Sums v[i] over the warp for each of kCount values (8, 16 or 32).  Afterwards
+// v[0] of lane l is the sum of the value that the lane's bits spell from the
+// top.
 template <int kCount>
 __device__ __forceinline__ void transpose_sum(float (&v)[kCount], int lane) {
   int count = kCount;
@@ -111,11 +83,11 @@ __device__ __forceinline__ void transpose_sum(float (&v)[kCount], int lane) {
 
 constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
 
-template <typename T, int kRows, int E, bool kVec>
+template <typename T, int kRows>
 __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a) {
   constexpr int kSums = kTile * kRows;  // value index: row * kTile + key
-  constexpr int kHeld = kSums > 32 ? kSums / 32 : 1;
-  constexpr int kWidth = 32 * E;
+  constexpr int E = kElements, kWidth = kPagedMaxHeadDim;
+  static_assert(kSums <= 32, "a lane for each score");
   __shared__ float weights[kWarps][kRows][kTile];
   __shared__ float rescale[kWarps][kRows];
   __shared__ PagedParts<kWarps, kRows> parts;
@@ -146,7 +118,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
   // Which row's score this lane holds after transpose_sum: the value index is
   // spelled by the lane's bits from the top.
   constexpr int kLogSums = log2_of(kSums);
-  const int index = kLogSums >= 5 ? lane << (kLogSums - 5) : lane >> (5 - kLogSums);
+  const int index = lane >> (5 - kLogSums);
   const int my_row = index / kTile, my_key = index % kTile;
 
   while (w < limit) {
@@ -170,7 +142,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
     float qr[kRows][E], o[kRows][E];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      load_row<T, E, kVec>(r < unit.rows ? q + sequence * a.q_batch +
+      load_row<T>(r < unit.rows ? q + sequence * a.q_batch +
                                                (unit.first_head + r) * a.q_head
                                          : nullptr,
                            a.head_dim, lane, qr[r]);
@@ -202,9 +174,9 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
       for (int j = 0; j < kTile; ++j) {
         k_place[j] = __shfl_sync(kFullMask, place, j);
         const int64_t v_place = __shfl_sync(kFullMask, place, 8 + j);
-        load_row<T, E, kVec>(k_place[j] >= 0 ? k_head + k_place[j] : nullptr, a.head_dim, lane,
+        load_row<T>(k_place[j] >= 0 ? k_head + k_place[j] : nullptr, a.head_dim, lane,
                              kr[j]);
-        load_row<T, E, kVec>(v_place >= 0 ? v_head + v_place : nullptr, a.head_dim, lane, vr[j]);
+        load_row<T>(v_place >= 0 ? v_head + v_place : nullptr, a.head_dim, lane, vr[j]);
       }
       float s[kSums];
 #pragma unroll
@@ -217,16 +189,12 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
           s[r * kTile + j] = dot;
         }
       transpose_sum(s, lane);
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        const bool there = __shfl_sync(kFullMask, place, my_key + i) >= 0;
-        s[i] = there ? s[i] * a.scale_log2 : -INFINITY;
-        top = fmaxf(top, s[i]);
-      }
+      const bool there = __shfl_sync(kFullMask, place, my_key) >= 0;
+      const float score = there ? s[0] * a.scale_log2 : -INFINITY;
+      float top = score;
       // The lanes that hold one row differ in these bits.
-      constexpr int kRowLanes = kRows >= 4 ? 32 / kRows : 8;
-      constexpr int kFirst = kRows >= 4 ? 1 : 4 / kRows;
+      constexpr int kRowLanes = 8;
+      constexpr int kFirst = 4 / kRows;
 #pragma unroll
       for (int x = 1; x < kRowLanes; x <<= 1)
         top = fmaxf(top, __shfl_xor_sync(kFullMask, top, x * kFirst));
@@ -234,15 +202,10 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
       const float base_m = m_new == -INFINITY ? 0.0f : m_new;  // no key so far: all weights 0
       const float alpha = paged_exp2(m - base_m);
       __syncwarp();  // the previous tile's weights have been read
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        const float p = paged_exp2(s[i] - base_m);
-        weights[warp][my_row][my_key + i] = p;
-        sum += p;
-      }
+      const float weight = paged_exp2(score - base_m);
+      weights[warp][my_row][my_key] = weight;
       if (my_key == 0) rescale[warp][my_row] = alpha;
-      l = l * alpha + sum;
+      l = l * alpha + weight;
       m = m_new;
       __syncwarp();
 #pragma unroll
@@ -261,8 +224,8 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
 
     // Every lane that holds a row has its maximum; the sum is over the lanes
     // that hold different keys of it.
-    constexpr int kRowLanes = kRows >= 4 ? 32 / kRows : 8;
-    constexpr int kFirst = kRows >= 4 ? 1 : 4 / kRows;
+    constexpr int kRowLanes = 8;
+    constexpr int kFirst = 4 / kRows;
 #pragma unroll
     for (int x = 1; x < kRowLanes; x <<= 1) l += __shfl_xor_sync(kFullMask, l, x * kFirst);
     constexpr int kLanesOfRow = 32 / kRows;  // lane of row r: the first of these
@@ -275,7 +238,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
                        (static_cast<int64_t>(sequence) * a.heads + unit.first_head + r) * a.head_dim;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const int d = column<E, kVec>(lane, e);
+          const int d = lane + 32 * e;
           if (d < a.head_dim) st_out(dst + d, length == 0 ? 0.0f : o[r][e] / sum);
         }
       }
@@ -296,7 +259,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
       if (r >= unit.rows) continue;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const int d = column<E, kVec>(lane, e);
+        const int d = lane + 32 * e;
         if (d < a.head_dim) part[r * pitch + d] = o[r][e];
       }
     }
@@ -306,16 +269,17 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
   }
   if (reported != 0) watchdog_trip(a.watchdog, reported);
   __syncthreads();
-  paged_merge<T, kWarps, kRows, kRows * kWidth, kWidth, kVec ? 4 : 1>(a, parts, rows);
+  paged_merge<T, kWarps, kRows, kRows * kWidth, kWidth, 1>(a, parts, rows);
 }
 
-template <typename T, int kRows, int E, bool kVec>
-int launch_simt(PagedArgs a, int grid_ctas, cudaStream_t stream) {
-  paged_scratch(&a, grid_ctas, kWarps, kRows);
-  constexpr size_t kShared = sizeof(float) * kWarps * kRows * 32 * E;
+template <typename T, int kRows>
+int launch_simt(PagedArgs a, cudaStream_t stream) {
+  const int grid = paged_grid(a, paged_grid_limit(), kTile, kWarps, kRows);
+  paged_scratch(&a, grid, kWarps, kRows);
+  constexpr size_t kShared = sizeof(float) * kWarps * kRows * kPagedMaxHeadDim;
   static_assert(kShared <= 40 * 1024, "fits without an opt-in");
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(grid_ctas);
+  config.gridDim = dim3(grid);
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = kShared;
   config.stream = stream;
@@ -324,29 +288,20 @@ int launch_simt(PagedArgs a, int grid_ctas, cudaStream_t stream) {
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
-  cudaError_t error = cudaLaunchKernelEx(&config, paged_simt_kernel<T, kRows, E, kVec>, a);
-  if (error == cudaSuccess && grid_ctas > 1)
-    error = launch_join<T, kTile, kWarps, kRows>(a, grid_ctas, stream);
+  cudaError_t error = cudaLaunchKernelEx(&config, paged_simt_kernel<T, kRows>, a);
+  if (error == cudaSuccess && grid > 1)
+    error = launch_join<T, kTile, kWarps, kRows>(a, grid, stream);
   return error != cudaSuccess ? error : cudaGetLastError();
 }
 
-template <typename T, int E, bool kVec>
-int pick_rows(const PagedArgs& a, int grid_ctas, cudaStream_t stream) {
-  if (a.group == 1) return launch_simt<T, 1, E, kVec>(a, grid_ctas, stream);
-  if (a.group == 2) return launch_simt<T, 2, E, kVec>(a, grid_ctas, stream);
-  // A lane holds rows * E elements of q and of the output each.
-  if (a.group <= 4 || E == 8) return launch_simt<T, 4, E, kVec>(a, grid_ctas, stream);
-  return launch_simt<T, 8, E == 8 ? 4 : E, kVec>(a, grid_ctas, stream);
-}
-
-bool aligned_rows(const PagedArgs& a, size_t element, int vector) {
-  const size_t bytes = element * vector;
+bool aligned_rows(const PagedArgs& a, size_t element) {
+  const int vector = 16 / static_cast<int>(element);
   const int64_t strides[] = {a.q_batch, a.q_head, a.k_page, a.k_token, a.k_head,
                              a.v_page,  a.v_token, a.v_head, a.head_dim};
   for (int64_t s : strides)
     if (s % vector != 0) return false;
   for (const void* p : {a.q, a.k, a.v, static_cast<const void*>(a.out)})
-    if (reinterpret_cast<std::uintptr_t>(p) % bytes != 0) return false;
+    if (!aligned16(p)) return false;
   return true;
 }
 
@@ -395,18 +350,13 @@ int paged_attention(const void* q, int64_t q_batch, int64_t q_head, const opl_kv
   a.partial = static_cast<float*>(workspace);
   a.watchdog = watchdog_word();
   if (a.watchdog == nullptr) return cudaErrorInvalidDevice;
-  const bool vec = sizeof(T) == 4 && aligned_rows(a, sizeof(T), 4);
-  if constexpr (sizeof(T) == 2) {
-    if (aligned_rows(a, sizeof(T), 8)) return paged_attention_mma<T>(a, stream);
+  if (aligned_rows(a, sizeof(T))) {
+    if constexpr (sizeof(T) == 4)
+      return paged_attention_f32(a, stream);
+    else
+      return paged_attention_mma<T>(a, stream);
   }
-  const int grid = paged_grid(a, paged_grid_limit(), kTile, kWarps, a.group <= 4 ? a.group : 4);
-  if constexpr (sizeof(T) == 4) {
-    if (vec && a.head_dim <= 64) return pick_rows<T, 2, true>(a, grid, stream);
-    if (vec && a.head_dim <= 128) return pick_rows<T, 4, true>(a, grid, stream);
-    if (vec) return pick_rows<T, 8, true>(a, grid, stream);
-  }
-  if (a.group == 1) return launch_simt<T, 1, 8, false>(a, grid, stream);
-  return launch_simt<T, 4, 8, false>(a, grid, stream);
+  return a.group == 1 ? launch_simt<T, 1>(a, stream) : launch_simt<T, 4>(a, stream);
 }
 
 }  // namespace

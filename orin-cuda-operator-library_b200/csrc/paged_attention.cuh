@@ -409,9 +409,10 @@ inline size_t paged_scratch_bytes(int group, int head_dim) {
   return ctas * rows * ((2 + kPagedMaxWarps) * sizeof(float) * head_dim + 2 * sizeof(float2));
 }
 
-// The tensor-core kernel: 16-bit types, head_dim a multiple of 8, addresses
-// and strides multiples of 16 bytes.
+// The streaming kernels: head_dim a multiple of 16 bytes, addresses and strides
+// too.
 template <typename T>
-int paged_attention_mma(PagedArgs a, cudaStream_t stream);
+int paged_attention_mma(const PagedArgs& a, cudaStream_t stream);
+int paged_attention_f32(const PagedArgs& a, cudaStream_t stream);
 
 }  // namespace opl
