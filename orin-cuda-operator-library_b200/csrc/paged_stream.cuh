@@ -25,6 +25,8 @@
 // runs once: it is kept short, and rolled.
 #pragma once
 
+#include <atomic>
+
 #include "paged_attention.cuh"
 #include "tc_common.cuh"
 #include "tmap.cuh"
@@ -391,9 +393,17 @@ int launch_stream(const PagedArgs& a, const CUtensorMap& k_map, const CUtensorMa
                   const MapOrder& order, int grid, cudaStream_t stream) {
   constexpr auto kernel = paged_stream_kernel<Policy, kTma, kWarps, kStages>;
   constexpr size_t kShared = Ring<Policy, kWarps, kStages>::kShared;
-  cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           static_cast<int>(kShared));
-  if (error != cudaSuccess) return error;
+  // Once a device: the call takes a microsecond of the host's time.
+  static std::atomic<uint64_t> allowed{0};
+  const int device = current_device();
+  const uint64_t bit = device >= 0 && device < 64 ? uint64_t{1} << device : 0;
+  cudaError_t error = cudaSuccess;
+  if ((allowed.load(std::memory_order_relaxed) & bit) == 0) {
+    error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(kShared));
+    if (error != cudaSuccess) return error;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(grid);
   config.blockDim = dim3(32 * kWarps);
