@@ -88,8 +88,14 @@ __device__ __forceinline__ PagedTotal paged_start(const PagedArgs& a, int grid_c
   // sequences, beyond that (1024: 68 against 74 us for the call) sums of 32 that
   // the warp loads together.
   uint32_t mine = 0;
-  int per = (a.batch + 31) / 32;
-  if (per <= 16) {
+  int per = (a.batch + 31) / 32, raw = 0;
+  if (per == 1) {
+    if (lane < a.batch) {
+      raw = ld_int(a.seq_lens + lane);
+      mine = key_tiles(
+          readable_length(raw, a.max_pages, static_cast<int>(a.page_size.divisor)), kTile);
+    }
+  } else if (per <= 16) {
 #pragma unroll 4
     for (int i = 0; i < per; ++i) {
       const int b = lane * per + i;
@@ -119,10 +125,18 @@ __device__ __forceinline__ PagedTotal paged_start(const PagedArgs& a, int grid_c
   // The lane whose sequences hold it, then the sequence among them.
   const int owner = __popc(__ballot_sync(kFullMask, end <= wanted));
   uint32_t before = __shfl_sync(kFullMask, end - mine, owner);
+  if (per == 1) {
+    start->sequence = owner;
+    start->raw_length = __shfl_sync(kFullMask, raw, owner);
+    start->length =
+        readable_length(start->raw_length, a.max_pages, static_cast<int>(a.page_size.divisor));
+    start->before = before;
+    return total;
+  }
   for (int i = 0; i < per; i += 32) {
     const int b = owner * per + i + lane;
     const bool there = i + lane < per && b < a.batch;
-    const int raw = there ? ld_int(a.seq_lens + b) : 0;
+    raw = there ? ld_int(a.seq_lens + b) : 0;
     const int length = readable_length(raw, a.max_pages, static_cast<int>(a.page_size.divisor));
     const uint32_t tiles = there ? key_tiles(length, kTile) : 0;
     const uint32_t upto = before + warp_prefix(tiles, lane);
@@ -203,6 +217,8 @@ template <int kWarps, int kRows>
 struct PagedParts {
   PartRecord records[kWarps][2];
   float m[kWarps][2][kRows], l[kWarps][2][kRows];  // log2 domain; sums
+  float weight[kWarps][2][kRows];                  // of the part in its unit
+  float top[kWarps][2][kRows], sum[kWarps][2][kRows];  // of the unit
 };
 
 // Joins the parts that the CTA's warps left, after a __syncthreads, and writes
@@ -210,7 +226,7 @@ struct PagedParts {
 // partial slots.  The parts' rows lie at rows + warp * kStride + row * kPitch
 // (floats), or in the spill of the warp.
 template <typename T, int kWarps, int kRows, int kStride, int kPitch, int kWidth>
-__device__ __forceinline__ void paged_merge(const PagedArgs& a, const PagedParts<kWarps, kRows>& parts,
+__device__ __forceinline__ void paged_merge(const PagedArgs& a, PagedParts<kWarps, kRows>& parts,
                                             const float* rows) {
   static_assert(kWarps <= 16, "a lane for each part");
   const int lane = threadIdx.x & 31;
@@ -222,56 +238,93 @@ __device__ __forceinline__ void paged_merge(const PagedArgs& a, const PagedParts
   }
   const uint32_t all = __ballot_sync(kFullMask, present);
   const uint32_t first = __ballot_sync(kFullMask, starts);
-  const int pieces = a.head_dim / kWidth;
-  // A few units: all threads on each.  Many, of short sequences: a warp each.
+  // A thread for each part and row: the part's weight in its unit.
+  const auto start_of = [&](int part) {  // the first part of the unit
+    return 31 - __clz(first & ((2u << part) - 1));
+  };
+  for (int i = threadIdx.x; i < 2 * kWarps * a.row_cap; i += 32 * kWarps) {
+    const int part = i % (2 * kWarps), row = i / (2 * kWarps);
+    if ((all >> part & 1u) == 0) continue;
+    const uint32_t mine = parts_of_unit(all, first, start_of(part));
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 4
+    for (int b = 0; b < kWarps; ++b) {  // a warp has at most one part of a unit
+      const uint32_t kinds = mine >> (2 * b) & 3u;
+      if (kinds != 0) top = fmaxf(top, parts.m[b][kinds >> 1][row]);
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+    for (int b = 0; b < kWarps; ++b) {
+      const uint32_t kinds = mine >> (2 * b) & 3u;
+      if (kinds != 0)
+        sum = fmaf(paged_exp2(parts.m[b][kinds >> 1][row] - base), parts.l[b][kinds >> 1][row], sum);
+    }
+    parts.weight[part >> 1][part & 1][row] =
+        paged_exp2(parts.m[part >> 1][part & 1][row] - base);
+    parts.top[part >> 1][part & 1][row] = top;
+    parts.sum[part >> 1][part & 1][row] = sum;
+  }
+  __syncthreads();
+  const int pieces = a.head_dim / kWidth, warp = threadIdx.x >> 5;
+  // A few units: the warps share the rows of each.  Many, of short sequences: a
+  // warp each.
   const bool together = __popc(first) <= 2;
+  constexpr int kAtOnce = 4;  // rows whose loads do not wait for one another
   int turn = 0;
   for (uint32_t left = first; left != 0; left &= left - 1, ++turn) {
-    if (!together && turn % kWarps != static_cast<int>(threadIdx.x >> 5)) continue;
+    if (!together && turn % kWarps != warp) continue;
     const int start = __ffs(left) - 1;
     const uint32_t mine = parts_of_unit(all, first, start);
     const int last = 31 - __clz(mine);
     const PartRecord& r = parts.records[start >> 1][start & 1];
     const bool whole = r.begin == 0 && parts.records[last >> 1][last & 1].end == r.tiles;
     const PagedUnit unit = paged_unit<kRows>(a, r.unit);
-    for (int i = together ? threadIdx.x : lane; i < unit.rows * pieces;
-         i += together ? 32 * kWarps : 32) {
-      const int row = i / pieces, d = (i - row * pieces) * kWidth;
-      // A warp has at most one part of a unit.
-      float top = -INFINITY;
-#pragma unroll 4
-      for (int b = 0; b < kWarps; ++b) {
-        const uint32_t kinds = mine >> (2 * b) & 3u;
-        if (kinds != 0) top = fmaxf(top, parts.m[b][kinds >> 1][row]);
-      }
-      const float base = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f, out[kWidth] = {};
-#pragma unroll 4
-      for (int b = 0; b < kWarps; ++b) {
-        const uint32_t kinds = mine >> (2 * b) & 3u;
-        if (kinds == 0) continue;
-        const int kind = kinds >> 1;
-        float v[kWidth];
-        ld_row(parts.records[b][kind].spilled == 0
-                   ? rows + b * kStride + row * kPitch + d
-                   : a.spill + ((static_cast<int64_t>(blockIdx.x) * kWarps + b) * a.row_cap + row) *
-                                   a.head_dim + d,
-               v);
-        const float f = paged_exp2(parts.m[b][kind][row] - base);
-        sum = fmaf(f, parts.l[b][kind][row], sum);
+    const int step = together ? kWarps : 1;
+    for (int row = together ? warp : 0; row < unit.rows; row += kAtOnce * step) {
+      for (int d = lane * kWidth; d < pieces * kWidth; d += 32 * kWidth) {
+        float out[kAtOnce][kWidth] = {};
+#pragma unroll 2
+        for (int b = 0; b < kWarps; ++b) {
+          const uint32_t kinds = mine >> (2 * b) & 3u;
+          if (kinds == 0) continue;
+          const int kind = kinds >> 1;
+          const bool spilled = parts.records[b][kind].spilled != 0;
+          const float* const src =
+              spilled ? a.spill + (static_cast<int64_t>(blockIdx.x) * kWarps + b) * a.row_cap * a.head_dim
+                      : rows + b * kStride;
+          const int pitch = spilled ? a.head_dim : kPitch;
+          float v[kAtOnce][kWidth];
 #pragma unroll
-        for (int e = 0; e < kWidth; ++e) out[e] = fmaf(f, v[e], out[e]);
-      }
-      if (whole) {
+          for (int q = 0; q < kAtOnce; ++q)
+            if (row + q * step < unit.rows) ld_row(src + (row + q * step) * pitch + d, v[q]);
 #pragma unroll
-        for (int e = 0; e < kWidth; ++e) out[e] = __fdividef(out[e], sum);
-        st_row(static_cast<T*>(a.out) +
-                   (static_cast<int64_t>(r.sequence) * a.heads + unit.first_head + row) * a.head_dim + d,
-               out);
-      } else {
-        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (r.begin == 0 ? 1 : 0);
-        st_row(a.partial + (slot * a.row_cap + row) * a.head_dim + d, out);
-        if (d == 0) a.partial_ml[slot * a.row_cap + row] = make_float2(top, sum);
+          for (int q = 0; q < kAtOnce; ++q) {
+            if (row + q * step >= unit.rows) continue;
+            const float f = parts.weight[b][kind][row + q * step];
+#pragma unroll
+            for (int e = 0; e < kWidth; ++e) out[q][e] = fmaf(f, v[q][e], out[q][e]);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+          const int at = row + q * step;
+          if (at >= unit.rows) continue;
+          const float sum = parts.sum[start >> 1][start & 1][at];
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < kWidth; ++e) out[q][e] = __fdividef(out[q][e], sum);
+            st_row(static_cast<T*>(a.out) +
+                       (static_cast<int64_t>(r.sequence) * a.heads + unit.first_head + at) * a.head_dim +
+                       d,
+                   out[q]);
+          } else {
+            const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (r.begin == 0 ? 1 : 0);
+            st_row(a.partial + (slot * a.row_cap + at) * a.head_dim + d, out[q]);
+            if (d == 0)
+              a.partial_ml[slot * a.row_cap + at] =
+                  make_float2(parts.top[start >> 1][start & 1][at], sum);
+          }
+        }
       }
     }
   }

@@ -277,11 +277,8 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     if (same || out.sequence + 1 < a.batch)
       policy.fetch_query(a, same ? out.sequence : out.sequence + 1, same ? out.unit + 1 : 0);
   };
-  if (to_read > 0) {
-    policy.fetch_query(a, out.sequence, out.unit);
-    policy.start(a, out.sequence, out.unit);
-    fetch_next_query();
-  }
+  if (to_read > 0) policy.fetch_query(a, out.sequence, out.unit);
+  bool fresh = true;  // the next tile read is its segment's first
 
   // Step s copies tile s and, once kStages - 1 tiles are on their way, reads
   // tile s - (kStages - 1).  (One loop for the first steps and the others:
@@ -318,6 +315,11 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     const uint32_t stage = ring_address + slot_out * S::kStageBytes;
     if (++slot_out == kStages) slot_out = 0, parity ^= 1u;
 
+    if (fresh) {
+      fresh = false;
+      policy.start(a, out.sequence, out.unit);
+      fetch_next_query();
+    }
     policy.step(a, stage, stage + S::kKeyBytes, there[0]);
 
     --to_read;
@@ -350,8 +352,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     if (to_read > 0) {
       advance(out);
       begin = 0;
-      policy.start(a, out.sequence, out.unit);
-      fetch_next_query();
+      fresh = true;
     }
   }
   if (reported != 0) watchdog_trip(a.watchdog, reported);
