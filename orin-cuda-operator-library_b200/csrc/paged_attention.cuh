@@ -443,7 +443,7 @@ inline int paged_grid(const PagedArgs& a, int limit, int tile, int warps, int un
   return active_ctas(tiles * units, limit, warps);
 }
 
-constexpr int kPagedMaxRows = 16, kPagedMaxWarps = 8;
+constexpr int kPagedMaxRows = 16, kPagedMaxWarps = 8;  // at two CTAs a SM
 
 // Lays the scratch out; its size is that of the largest launch.
 inline void paged_scratch(PagedArgs* a, int grid, int warps, int rows) {

@@ -313,9 +313,10 @@ struct MmaPolicy {
 
 template <typename T, int kRows>
 int pick_dim(const PagedArgs& a, cudaStream_t stream) {
-  // Warps and stages by head size: 64: 8 x 3 (x 6: 110 against 99 us for 200,000
-  // keys); 128: see paged_stream.cuh; over 128 four warps, for their registers.
-  if (a.head_dim <= 64) return paged_stream<MmaPolicy<T, 64, kRows>, 8, 3>(a, stream);
+  // Warps and stages by head size.  64: 12 x 2 at 168 registers (100,000 keys, 8
+  // heads: 71 us; 8 x 3, 82 us; 16 x 2 the same as 12).  128: see
+  // paged_stream.cuh.  Over 128 four warps, for their registers.
+  if (a.head_dim <= 64) return paged_stream<MmaPolicy<T, 64, kRows>, 12, 2>(a, stream);
   if (a.head_dim <= 128) return paged_stream<MmaPolicy<T, 128, kRows>, 8, 2>(a, stream);
   if (a.head_dim <= 192) return paged_stream<MmaPolicy<T, 192, kRows>, 4, 3>(a, stream);
   return paged_stream<MmaPolicy<T, 256, kRows>, 4, 2>(a, stream);

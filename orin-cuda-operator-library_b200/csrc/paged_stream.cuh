@@ -75,6 +75,8 @@ struct Ring {
   static_assert(kStageBytes % 1024 == 0 && Policy::kWarpShared % 16 == 0, "alignment");
   static_assert(Policy::kRows * kPitch * 4 <= kBytes, "a warp merges through its own ring");
   static_assert(kShared <= 222 * 1024, "beside the static arrays");
+  // paged_scratch_bytes, with one CTA a SM.
+  static_assert(2 + kWarps <= 2 * (2 + kPagedMaxWarps) && Policy::kRows <= kPagedMaxRows, "scratch");
 };
 
 // Copies are made by the TMA unit, or by the lanes (kTma false).
