@@ -214,7 +214,7 @@ int opl_kv_append_bf16(const opl_bf16_t* q, int64_t q_token, int64_t q_head, con
                        const opl_rope_spec* rope, opl_stream_t stream);
 
 /* Attention of one new token per sequence: q and out are [batch, heads,
- * head_dim] (out contiguous), query head h reads key-value head
+ * head_dim] (out contiguous, overlapping nothing), query head h reads key-value head
  * h / (heads / kv_heads), and sequence b has seq_lens[b] keys, key j in page
  * block_table[b * table_row + j / page_size].  Softmax over scale * q.K in
  * FP32; the result is rounded once to the tensors' type.  A sequence of length

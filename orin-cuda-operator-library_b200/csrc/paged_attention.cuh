@@ -49,9 +49,15 @@ __device__ __forceinline__ int ld_int(const int* p) {
   return r;
 }
 
-__device__ __forceinline__ int paged_length(const PagedArgs& a, int sequence) {
-  return readable_length(ld_int(a.seq_lens + sequence), a.max_pages,
-                         static_cast<int>(a.page_size.divisor));
+// The same from L2: for a launch that may share its SM's L1 with an earlier one.
+__device__ __forceinline__ int ld_int_l2(const int* p) {
+  int r;
+  asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(r) : "l"(p));
+  return r;
+}
+
+__device__ __forceinline__ int readable(const PagedArgs& a, int raw_length) {
+  return readable_length(raw_length, a.max_pages, static_cast<int>(a.page_size.divisor));
 }
 
 struct PagedTotal {
@@ -80,10 +86,14 @@ __device__ __forceinline__ uint32_t warp_prefix(uint32_t x, int lane) {  // with
 // this is the start of the launch, where a barrier and what it orders would
 // cost more than the repeated loads.  kUnitWarps: warps of a CTA of the main
 // launch.  The sums fit 32 bits (see the limit on the cache's capacity).
-template <int kTile, int kUnitWarps, typename Place>
+template <int kTile, int kUnitWarps, bool kFromL2, typename Place>
 __device__ __forceinline__ PagedTotal paged_start(const PagedArgs& a, int grid_ctas,
                                                   PagedStart* start, Place place) {
   const int lane = threadIdx.x & 31;
+  const auto raw_of = [&](int b) {
+    return kFromL2 ? ld_int_l2(a.seq_lens + b) : ld_int(a.seq_lens + b);
+  };
+  const auto tiles_of = [&](int b) -> uint32_t { return key_tiles(readable(a, raw_of(b)), kTile); };
   // Lane x adds up the tiles of `per` sequences: its own loads up to 512
   // sequences, beyond that (1024: 68 against 74 us for the call) sums of 32 that
   // the warp loads together.
@@ -91,23 +101,21 @@ __device__ __forceinline__ PagedTotal paged_start(const PagedArgs& a, int grid_c
   int per = (a.batch + 31) / 32, raw = 0;
   if (per == 1) {
     if (lane < a.batch) {
-      raw = ld_int(a.seq_lens + lane);
-      mine = key_tiles(
-          readable_length(raw, a.max_pages, static_cast<int>(a.page_size.divisor)), kTile);
+      raw = raw_of(lane);
+      mine = key_tiles(readable(a, raw), kTile);
     }
   } else if (per <= 16) {
 #pragma unroll 4
     for (int i = 0; i < per; ++i) {
       const int b = lane * per + i;
-      if (b < a.batch) mine += key_tiles(paged_length(a, b), kTile);
+      if (b < a.batch) mine += tiles_of(b);
     }
   } else {
     per = 32 * ((per + 31) / 32);
     int adder = 0, left = per;
 #pragma unroll 8
     for (int b = lane; b - lane < a.batch; b += 32) {
-      const uint32_t sum =
-          __reduce_add_sync(kFullMask, b < a.batch ? key_tiles(paged_length(a, b), kTile) : 0u);
+      const uint32_t sum = __reduce_add_sync(kFullMask, b < a.batch ? tiles_of(b) : 0u);
       if (lane == adder) mine += sum;
       if ((left -= 32) == 0) left = per, ++adder;
     }
@@ -128,16 +136,15 @@ __device__ __forceinline__ PagedTotal paged_start(const PagedArgs& a, int grid_c
   if (per == 1) {
     start->sequence = owner;
     start->raw_length = __shfl_sync(kFullMask, raw, owner);
-    start->length =
-        readable_length(start->raw_length, a.max_pages, static_cast<int>(a.page_size.divisor));
+    start->length = readable(a, start->raw_length);
     start->before = before;
     return total;
   }
   for (int i = 0; i < per; i += 32) {
     const int b = owner * per + i + lane;
     const bool there = i + lane < per && b < a.batch;
-    raw = there ? ld_int(a.seq_lens + b) : 0;
-    const int length = readable_length(raw, a.max_pages, static_cast<int>(a.page_size.divisor));
+    raw = there ? raw_of(b) : 0;
+    const int length = readable(a, raw);
     const uint32_t tiles = there ? key_tiles(length, kTile) : 0;
     const uint32_t upto = before + warp_prefix(tiles, lane);
     const uint32_t passed = __ballot_sync(kFullMask, upto <= wanted);
@@ -341,32 +348,42 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
   constexpr int kHeld = kPagedMaxHeadDim / (32 * kWidth);  // pieces of a lane
   __shared__ float warp_top[kJoinWarps], warp_sum[kJoinWarps];
   __shared__ float rows[kJoinWarps][kPagedMaxHeadDim];
-  const int cta = blockIdx.x;
+  __shared__ int found_sequence, found_unit, found_parts;
+  const int cta = blockIdx.x, row = blockIdx.y;
   // The main launch waits for everything before it and only then lets this one
   // be scheduled, and it leaves the lengths alone: they can be read while it
-  // still runs.
-  const auto cta_begin = [](const PagedTotal& t, int64_t index) {
-    return t.ranges.begin(kUnitWarps * index);
-  };
-  PagedStart start;
-  const PagedTotal total = paged_start<kUnitTile, kUnitWarps>(
-      a, grid_ctas, &start, [&](const PagedTotal& t) -> int64_t {
-        return cta + 1 < t.ctas ? cta_begin(t, cta + 1) - 1 : -1;
-      });
-  if (cta + 1 >= total.ctas) return;
-  const int64_t at = cta_begin(total, cta + 1) - 1;  // the CTA's last tile
-  const int sequence = start.sequence;
-  const int tiles = key_tiles(start.length, kUnitTile);
-  const TilePlace last = place_of(at, start.before, tiles, a.units.divisor);
-  if (last.tile + 1 == tiles) return;  // not cut here
-  const int64_t unit_begin = at - last.tile;
-  if (unit_begin < cta_begin(total, cta)) return;  // an earlier CTA starts it
-  const PagedUnit unit = paged_unit<kRows>(a, last.unit);
-  const int row = blockIdx.y;
+  // still runs.  One block waits for it in any case, so that this launch does
+  // not end, and the next one on the stream not begin, before it.
+  if (cta == 0 && row == 0) pdl_begin();
+  if (threadIdx.x < 32) {
+    const auto cta_begin = [](const PagedTotal& t, int64_t index) {
+      return t.ranges.begin(kUnitWarps * index);
+    };
+    PagedStart start = {};
+    const PagedTotal total = paged_start<kUnitTile, kUnitWarps, true>(
+        a, grid_ctas, &start, [&](const PagedTotal& t) -> int64_t {
+          return cta + 1 < t.ctas ? cta_begin(t, cta + 1) - 1 : -1;
+        });
+    int parts = 0, unit = 0;
+    if (cta + 1 < total.ctas) {
+      const int64_t at = cta_begin(total, cta + 1) - 1;  // the CTA's last tile
+      const int tiles = key_tiles(start.length, kUnitTile);
+      const TilePlace last = place_of(at, start.before, tiles, a.units.divisor);
+      const int64_t unit_begin = at - last.tile;
+      // Cut here, and not started by an earlier CTA.
+      if (last.tile + 1 != tiles && unit_begin >= cta_begin(total, cta)) {
+        unit = last.unit;
+        parts = static_cast<int>(total.ranges.holder(unit_begin + tiles - 1) / kUnitWarps) - cta + 1;
+      }
+    }
+    if (threadIdx.x == 0) found_sequence = start.sequence, found_unit = unit, found_parts = parts;
+  }
+  __syncthreads();
+  const int parts = found_parts, sequence = found_sequence;
+  if (parts == 0) return;
+  const PagedUnit unit = paged_unit<kRows>(a, found_unit);
   if (row >= unit.rows) return;
   pdl_begin();  // the main launch's parts
-  const int parts =
-      static_cast<int>(total.ranges.holder(unit_begin + tiles - 1) / kUnitWarps) - cta + 1;
   const auto part_row = [&](int p) {
     const int64_t slot = p == 0 ? 2 * static_cast<int64_t>(cta) + 1 : 2 * static_cast<int64_t>(cta + p);
     return slot * a.row_cap + row;

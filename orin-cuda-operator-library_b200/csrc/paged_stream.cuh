@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   if (lane < 2) parts.records[warp][lane] = PartRecord{};
   const int64_t range = int64_t{kWarps} * blockIdx.x + warp;
   PagedStart start;
-  const PagedTotal total = paged_start<kTile, kWarps>(
+  const PagedTotal total = paged_start<kTile, kWarps, false>(
       a, gridDim.x, &start, [range](const PagedTotal& x) -> int64_t {
         const int64_t at = x.ranges.begin(range);
         return static_cast<int>(blockIdx.x) < x.ctas && at < x.tiles ? at : -1;

@@ -545,6 +545,30 @@ def test_raw_helpers_on_another_stream(cuda):
     assert torch.equal(torch.nan_to_num(k2), torch.nan_to_num(cache.k))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("lens", [[9] * 2500, [700] * 90, [5000] * 3], ids=lambda x: f"{len(x)}x{x[0]}")
+def test_next_launch_may_overwrite_the_inputs(ops, cuda, dtype, lens):
+    """What follows on the stream may write over what the attention reads: no
+    launch begins before it has ended, whether units are cut between CTAs (a
+    second launch) or not (nothing for that launch to do)."""
+    cache = Paged(lens, 4, 64, 16, dtype, 61)
+    inv_freq = (10000.0 ** (-torch.arange(0, 64, 2, device="cuda") / 64)).float()
+    zero = torch.zeros(len(lens), dtype=torch.int64, device="cuda")
+    q = randn(gen(1), len(lens), 8, 64, dtype=dtype)
+    other = randn(gen(2), len(lens), 8, 64, dtype=dtype)
+    want = ops.paged_attention(q, cache.k, cache.v, cache.table, cache.seq_lens)
+    workspace = operatorlib.paged_attention_workspace(8, 4, 64, cuda)
+    outs = [torch.empty_like(q) for _ in range(6)]
+    buffers = [q.clone() for _ in outs]
+    torch.cuda.synchronize()
+    for out, buffer in zip(outs, buffers):
+        operatorlib.paged_attention_into(buffer, cache.k, cache.v, cache.table, cache.seq_lens,
+                                         out, workspace)
+        operatorlib.rope_into(other, buffer, zero, inv_freq)  # angle 0: a copy of `other`
+    for out, buffer in zip(outs, buffers):
+        assert torch.equal(out, want) and torch.equal(buffer, other)
+
+
 class Decoder:
     """A decoding loop's buffers for one layer: the calls of one step as a
     serving program makes them, and the same step from the formulas."""
