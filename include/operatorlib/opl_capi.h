@@ -138,8 +138,8 @@ int opl_attention_f16(const opl_half_t* q, const opl_half_t* k,
 /* Decoding with a paged key-value cache (no counterpart in the reference,
  * whose attention takes whole contiguous [B,H,S,D] tensors): rotary positions,
  * appending to the cache, attention of one new token over it.  Tensors may
- * have any strides (in elements) as long as head_dim is contiguous; head_dim
- * is at most 256.  Addresses and strides that are multiples of 16 bytes take
+ * have any strides (in elements, not negative) as long as head_dim is
+ * contiguous; head_dim is at most 256.  Addresses and strides that are multiples of 16 bytes take
  * the widest loads.  Indices that the device reads (slots, block table,
  * lengths) are checked there: a bad one is not followed, and its code is left
  * in the watchdog word (opl_read_and_clear_watchdog): 0x6b01 slot past the
@@ -220,7 +220,8 @@ int opl_kv_append_bf16(const opl_bf16_t* q, int64_t q_token, int64_t q_head, con
  * FP32; the result is rounded once to the tensors' type.  A sequence of length
  * 0 gives zeros.  Table entries past a sequence's pages are not read, and
  * neither are a page's tokens past its length.  Keys of a page outside the
- * cache are left out.  batch * max_pages * page_size is at most 2^34.
+ * cache are left out.  max_pages * page_size is at most 2^30, and batch times
+ * that at most 2^34.
  * `workspace` is 16-byte aligned device memory of at least the size that
  * opl_paged_attention_workspace gives; its contents do not matter and need not
  * be kept, but two calls that may overlap on the GPU need one each. */

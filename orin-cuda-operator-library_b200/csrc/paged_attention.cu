@@ -142,10 +142,9 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
     float qr[kRows][E], o[kRows][E];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      load_row<T>(r < unit.rows ? q + sequence * a.q_batch +
-                                               (unit.first_head + r) * a.q_head
-                                         : nullptr,
-                           a.head_dim, lane, qr[r]);
+      load_row<T>(
+          r < unit.rows ? q + sequence * a.q_batch + (unit.first_head + r) * a.q_head : nullptr,
+          a.head_dim, lane, qr[r]);
 #pragma unroll
       for (int e = 0; e < E; ++e) o[r][e] = 0.0f;
     }
@@ -169,13 +168,11 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
         }
       }
       float kr[kTile][E], vr[kTile][E];
-      int64_t k_place[kTile];
 #pragma unroll
       for (int j = 0; j < kTile; ++j) {
-        k_place[j] = __shfl_sync(kFullMask, place, j);
+        const int64_t k_place = __shfl_sync(kFullMask, place, j);
         const int64_t v_place = __shfl_sync(kFullMask, place, 8 + j);
-        load_row<T>(k_place[j] >= 0 ? k_head + k_place[j] : nullptr, a.head_dim, lane,
-                             kr[j]);
+        load_row<T>(k_place >= 0 ? k_head + k_place : nullptr, a.head_dim, lane, kr[j]);
         load_row<T>(v_place >= 0 ? v_head + v_place : nullptr, a.head_dim, lane, vr[j]);
       }
       float s[kSums];
@@ -316,6 +313,7 @@ int paged_attention(const void* q, int64_t q_batch, int64_t q_head, const opl_kv
       cache->kv_heads <= 0 || heads % cache->kv_heads != 0 || cache->head_dim <= 0 ||
       cache->head_dim > kPagedMaxHeadDim || !(scale - scale == 0.0f) ||
       reinterpret_cast<std::uintptr_t>(workspace) % 16 != 0 ||
+      static_cast<int64_t>(max_pages) * cache->page_size > kPagedMaxLength ||
       static_cast<int64_t>(max_pages) * cache->page_size > kPagedMaxKeys / batch)
     return cudaErrorInvalidValue;
   size_t needed = 0;

@@ -440,9 +440,10 @@ cudaError_t launch_join(const PagedArgs& a, int grid_ctas, cudaStream_t stream) 
                     grid_ctas);
 }
 
-// Keys that a block table may have room for, all sequences together: the
-// schedule counts tiles of 8 keys and more in 32 bits.
-constexpr int64_t kPagedMaxKeys = int64_t{1} << 34;
+// Keys that a block table may have room for: a sequence's (positions are int,
+// and tiles behind the last one are formed), and all sequences' together (the
+// schedule counts tiles of 8 keys and more in 32 bits).
+constexpr int64_t kPagedMaxLength = int64_t{1} << 30, kPagedMaxKeys = int64_t{1} << 34;
 
 // The most CTAs of a launch; the workspace is sized for them.
 inline int paged_grid_limit() { return 2 * sm_count(); }

@@ -401,8 +401,9 @@ Tensor op_paged_attention(const Tensor& q, const Tensor& k_cache, const Tensor& 
   TORCH_CHECK(seq_lens.dim() == 1 && seq_lens.size(0) == batch,
               "seq_lens must have one element a sequence");
   const int max_pages = as_positive_int(block_table.size(1), "block_table columns");
-  TORCH_CHECK(block_table.size(1) * cache.page_size <= (int64_t{1} << 34) / batch,
-              "block_table has room for more than 2^34 keys");
+  const int64_t room = block_table.size(1) * cache.page_size;
+  TORCH_CHECK(room <= int64_t{1} << 30 && room <= (int64_t{1} << 34) / batch,
+              "block_table has room for more than 2^30 keys a sequence, or 2^34 in all");
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(cache.head_dim));
   TORCH_CHECK(std::isfinite(static_cast<float>(s)), "scale must be finite");
   if (g_meta_call) return at::empty(q.sizes(), q.options());

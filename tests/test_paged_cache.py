@@ -89,7 +89,8 @@ def test_kv_append_refusals(suffix, change):
 @pytest.mark.parametrize("change", [
     dict(q=None), dict(out=None), dict(table=None), dict(lens=None), dict(workspace=None),
     dict(workspace=FAKE + 8), dict(bytes=16), dict(batch=0), dict(heads=0), dict(heads=5),
-    dict(max_pages=0), dict(max_pages=2 ** 29), dict(scale=float("nan")), dict(scale=float("inf")), dict(cache=None),
+    dict(max_pages=0), dict(max_pages=2 ** 26 + 1), dict(max_pages=2 ** 25, batch=33),
+    dict(scale=float("nan")), dict(scale=float("inf")), dict(cache=None),
     dict(cache=dict(k=None)), dict(cache=dict(v=None)), dict(cache=dict(pages=0)),
     dict(cache=dict(page_size=-1)), dict(cache=dict(kv_heads=0)), dict(cache=dict(head_dim=0)),
     dict(cache=dict(head_dim=257)),
@@ -229,7 +230,7 @@ def test_kv_append_op_refusals(ops, change, text):
     (dict(block_table=meta(5, 0, dtype=torch.int32)), "positive int32"),
     (dict(seq_lens=meta(5, dtype=torch.int64)), "seq_lens must be int32"),
     (dict(seq_lens=meta(4, dtype=torch.int32)), "one element a sequence"),
-    (dict(block_table=meta(5, 2 ** 28, dtype=torch.int32)), "more than 2\\^34"),
+    (dict(block_table=meta(5, 2 ** 26 + 1, dtype=torch.int32)), "2\\^30 keys a sequence"),
     (dict(scale=float("inf")), "scale must be finite"),
     (dict(scale=1e39), "scale must be finite"),
 ])
