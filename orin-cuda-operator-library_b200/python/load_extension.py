@@ -20,7 +20,8 @@ if str(_PKG_PARENT) not in sys.path:
 
 def load_operatorlib(verbose: bool = False) -> None:
     """Registers torch.ops.operatorlib.{reduce_sum, softmax, transpose,
-    rmsnorm, gemm, attention}; raises if the CUDA library is not built."""
+    rmsnorm, gemm, attention} and {rope, kv_append, paged_attention}; raises
+    if the CUDA library is not built."""
     import operatorlib
 
     operatorlib.load_operatorlib(verbose=verbose)
