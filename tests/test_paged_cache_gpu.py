@@ -333,7 +333,8 @@ def test_attention_page_sizes(ops, dtype, page):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=names)
 @pytest.mark.parametrize("lens", [[1], [7], [8], [9], [4097], [20011], [1, 20000, 3], [0], [0, 0, 0],
-                                  [0] * 20 + [5] + [0] * 20, list(range(300)), [1] * 700],
+                                  [0] * 20 + [5] + [0] * 20, list(range(300)), [1] * 700,
+                                  [i % 7 * 3 for i in range(2100)]],
                          ids=lambda x: f"{len(x)}x{max(x)}")
 def test_attention_lengths(ops, dtype, lens):
     """One token to long sequences, empty ones, ragged batches past one CTA's
