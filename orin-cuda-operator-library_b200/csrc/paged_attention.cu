@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
   __shared__ float weights[kWarps][kRows][kTile];
   __shared__ float rescale[kWarps][kRows];
   __shared__ PagedParts<kWarps, kRows> parts;
-  extern __shared__ __align__(16) float rows[];  // [kWarps][kRows][kWidth]
+  extern __shared__ __align__(16) float rows[];  // [2][kWarps][kRows][kWidth]
+  float* const heads = rows + kWarps * kRows * kWidth;
   pdl_begin();
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -241,12 +242,9 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
       }
       continue;
     }
-    // A part: to shared memory when the warp is done, else out of its way.
     const int kind = at.tile == 0 ? kTail : kHead;
-    const bool spilled = w < limit;
-    float* const part =
-        spilled ? a.spill + range * a.row_cap * a.head_dim : rows + warp * kRows * kWidth;
-    const int pitch = spilled ? a.head_dim : kWidth;
+    const bool aside = w < limit;
+    float* const part = (aside ? heads : rows) + warp * kRows * kWidth;
     if (lane % kLanesOfRow == 0 && my_row < unit.rows) {
       parts.m[warp][kind][my_row] = m;
       parts.l[warp][kind][my_row] = l;
@@ -257,24 +255,27 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int d = lane + 32 * e;
-        if (d < a.head_dim) part[r * pitch + d] = o[r][e];
+        if (d < a.head_dim) part[r * kWidth + d] = o[r][e];
       }
     }
     if (lane == 0)
       parts.records[warp][kind] = PartRecord{sequence, at.unit, tiles,  at.tile,
-                                             end,      opens && kind == kHead, spilled};
+                                             end,      opens && kind == kHead, aside};
   }
   if (reported != 0) watchdog_trip(a.watchdog, reported);
   __syncthreads();
-  paged_merge<T, kWarps, kRows, kRows * kWidth, kWidth, 1>(a, parts, rows);
+  paged_merge<T, kWarps, kRows, kRows * kWidth, kWidth, 1>(a, parts, rows, heads);
 }
 
 template <typename T, int kRows>
 int launch_simt(PagedArgs a, cudaStream_t stream) {
   const int grid = paged_grid(a, paged_grid_limit(), kTile, kWarps, kRows);
-  paged_scratch(&a, grid, kWarps, kRows);
-  constexpr size_t kShared = sizeof(float) * kWarps * kRows * kPagedMaxHeadDim;
-  static_assert(kShared <= 40 * 1024, "fits without an opt-in");
+  paged_scratch(&a, grid, kRows);
+  constexpr size_t kShared = sizeof(float) * 2 * kWarps * kRows * kPagedMaxHeadDim;
+  const cudaError_t allowed =
+      cudaFuncSetAttribute(paged_simt_kernel<T, kRows>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(kShared));
+  if (allowed != cudaSuccess) return allowed;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(grid);
   config.blockDim = dim3(kThreads);

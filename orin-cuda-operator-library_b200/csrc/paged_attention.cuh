@@ -31,7 +31,7 @@ struct PagedArgs {
   int row_cap;         // the most rows of a unit, min(group, the kernel's)
   float* partial;      // [ctas][2][row_cap][head_dim], not normalised
   float2* partial_ml;  // [ctas][2][row_cap]: maximum (log2 domain) and sum
-  float* spill;        // [ctas * warps][row_cap][head_dim]: heads of warps
+  float* aside;        // parts put aside that shared memory has no room for
   int* watchdog;
 };
 
@@ -197,7 +197,7 @@ __device__ __forceinline__ void st_row(T* p, const float (&x)[kWidth]) {
   }
 }
 
-// kWidth consecutive floats of shared or global memory, written by this CTA.
+// kWidth consecutive floats that this CTA has written.
 template <int kWidth>
 __device__ __forceinline__ void ld_row(const float* p, float (&x)[kWidth]) {
   if constexpr (kWidth == 4) {
@@ -230,11 +230,11 @@ struct PagedParts {
 
 // Joins the parts that the CTA's warps left, after a __syncthreads, and writes
 // each unit to the output or, when it reaches past the CTA, to the CTA's
-// partial slots.  The parts' rows lie at rows + warp * kStride + row * kPitch
-// (floats), or in the spill of the warp.
+// partial slots.  The parts' rows, kPitch floats each, lie at rows + warp *
+// kStride, or at heads + warp * kRows * kPitch when put aside.
 template <typename T, int kWarps, int kRows, int kStride, int kPitch, int kWidth>
 __device__ __forceinline__ void paged_merge(const PagedArgs& a, PagedParts<kWarps, kRows>& parts,
-                                            const float* rows) {
+                                            const float* rows, const float* heads) {
   static_assert(kWarps <= 16, "a lane for each part");
   const int lane = threadIdx.x & 31;
   bool present = false, starts = false;
@@ -295,15 +295,12 @@ __device__ __forceinline__ void paged_merge(const PagedArgs& a, PagedParts<kWarp
           const uint32_t kinds = mine >> (2 * b) & 3u;
           if (kinds == 0) continue;
           const int kind = kinds >> 1;
-          const bool spilled = parts.records[b][kind].spilled != 0;
-          const float* const src =
-              spilled ? a.spill + (static_cast<int64_t>(blockIdx.x) * kWarps + b) * a.row_cap * a.head_dim
-                      : rows + b * kStride;
-          const int pitch = spilled ? a.head_dim : kPitch;
+          const float* const src = parts.records[b][kind].aside != 0 ? heads + b * kRows * kPitch
+                                                                     : rows + b * kStride;
           float v[kAtOnce][kWidth];
 #pragma unroll
           for (int q = 0; q < kAtOnce; ++q)
-            if (row + q * step < unit.rows) ld_row(src + (row + q * step) * pitch + d, v[q]);
+            if (row + q * step < unit.rows) ld_row(src + (row + q * step) * kPitch + d, v[q]);
 #pragma unroll
           for (int q = 0; q < kAtOnce; ++q) {
             if (row + q * step >= unit.rows) continue;
@@ -461,23 +458,28 @@ inline int paged_grid(const PagedArgs& a, int limit, int tile, int warps, int un
   return active_ctas(tiles * units, limit, warps);
 }
 
-constexpr int kPagedMaxRows = 16, kPagedMaxWarps = 8;  // at two CTAs a SM
+constexpr int kPagedMaxRows = 16;
+
+// Floats of a CTA's parts put aside that do not fit beside 16 rows of more than
+// 192 columns, four warps.
+constexpr size_t kPagedHeadFloats = 4 * 16 * (kPagedMaxHeadDim + 4);
+inline bool heads_in_scratch(int group, int head_dim) { return group > 8 && head_dim > 192; }
 
 // Lays the scratch out; its size is that of the largest launch.
-inline void paged_scratch(PagedArgs* a, int grid, int warps, int rows) {
+inline void paged_scratch(PagedArgs* a, int grid, int rows) {
   a->parts = make_fast_div((a->group + rows - 1) / rows);
   a->units = make_fast_div(a->kv_heads * a->parts.divisor);
   a->row_cap = a->group < rows ? a->group : rows;
   const int64_t slots = static_cast<int64_t>(grid) * 2 * a->row_cap;
-  a->spill = a->partial + slots * a->head_dim;
-  a->partial_ml = reinterpret_cast<float2*>(
-      a->spill + static_cast<int64_t>(grid) * warps * a->row_cap * a->head_dim);
+  a->partial_ml = reinterpret_cast<float2*>(a->partial + slots * a->head_dim);
+  a->aside = reinterpret_cast<float*>(a->partial_ml + slots);
 }
 
 inline size_t paged_scratch_bytes(int group, int head_dim) {
   const size_t rows = group < kPagedMaxRows ? group : kPagedMaxRows;
-  const size_t ctas = paged_grid_limit();
-  return ctas * rows * ((2 + kPagedMaxWarps) * sizeof(float) * head_dim + 2 * sizeof(float2));
+  return 2 * static_cast<size_t>(paged_grid_limit()) * rows *
+             (sizeof(float) * head_dim + sizeof(float2)) +
+         (heads_in_scratch(group, head_dim) ? sm_count() * kPagedHeadFloats * sizeof(float) : 0);
 }
 
 // The streaming kernels: head_dim a multiple of 16 bytes, addresses and strides

@@ -42,16 +42,19 @@ struct Ranges {
   }
   OPL_HD int64_t holder(int64_t tile) const {  // the range of a tile
     const int64_t longer = (each + 1) * more;
-    return tile < longer ? tile / (each + 1) : more + (tile - longer) / each;
+    return tile < longer ? quotient(tile, each + 1) : more + quotient(tile - longer, each);
+  }
+  // 64-bit divisions take hundreds of cycles.
+  static OPL_HD int64_t quotient(int64_t a, int64_t b) {
+    if (a >> 32 == 0 && b >> 32 == 0)
+      return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
   }
 };
 
 OPL_HD Ranges make_ranges(int64_t total, int count) {
   Ranges r;
-  // 64-bit divisions take hundreds of cycles at the start of every CTA.
-  r.each = total >> 32 == 0 ? static_cast<int64_t>(static_cast<uint32_t>(total) /
-                                                   static_cast<uint32_t>(count))
-                            : total / count;
+  r.each = Ranges::quotient(total, count);
   r.more = total - r.each * count;
   return r;
 }
@@ -68,11 +71,7 @@ struct TilePlace {
 OPL_HD TilePlace place_of(int64_t w, int64_t before, int tiles, int units) {
   const int64_t local = w - before * units;
   TilePlace p;
-  if (local >> 32 == 0) {
-    p.unit = static_cast<int>(static_cast<uint32_t>(local) / static_cast<uint32_t>(tiles));
-  } else {
-    p.unit = static_cast<int>(local / tiles);
-  }
+  p.unit = static_cast<int>(Ranges::quotient(local, tiles));
   p.tile = static_cast<int>(local - static_cast<int64_t>(p.unit) * tiles);
   return p;
 }
@@ -81,7 +80,7 @@ OPL_HD TilePlace place_of(int64_t w, int64_t before, int tiles, int units) {
 struct PartRecord {
   int sequence, unit, tiles, begin, end;
   int opens;    // a head with which the CTA's range begins
-  int spilled;  // lies in global memory, the warp's ring had more to do
+  int aside;    // a head with more of the warp's range behind it
 
   OPL_HD bool empty() const { return begin == end; }
 };

@@ -70,13 +70,18 @@ struct Ring {
   static constexpr int kStageBytes = 2 * kKeyBytes;
   static constexpr int kBytes = kStages * kStageBytes;  // of a warp
   static constexpr int kPitch = Policy::kDim + 4;       // of a merged row, in floats
+  // A part put aside, in shared memory but for 16 rows of 256 columns, whose
+  // kernel needs what is left for L1 (16/1 heads of 256: 31.0 against 34.3 us).
+  static constexpr bool kSharedHeads = Policy::kRows * Policy::kDim <= 16 * 192;
+  static constexpr int kHeadBytes = kSharedHeads ? Policy::kRows * kPitch * 4 : 0;
   static constexpr size_t kShared =
-      1024 + static_cast<size_t>(kWarps) * (kBytes + Policy::kWarpShared);
+      1024 + static_cast<size_t>(kWarps) * (kBytes + Policy::kWarpShared + kHeadBytes);
   static_assert(kStageBytes % 1024 == 0 && Policy::kWarpShared % 16 == 0, "alignment");
   static_assert(Policy::kRows * kPitch * 4 <= kBytes, "a warp merges through its own ring");
-  static_assert(kShared <= 222 * 1024, "beside the static arrays");
-  // paged_scratch_bytes, with one CTA a SM.
-  static_assert(2 + kWarps <= 2 * (2 + kPagedMaxWarps) && Policy::kRows <= kPagedMaxRows, "scratch");
+  static_assert(kShared <= 220 * 1024, "beside the static arrays");
+  static_assert(Policy::kRows <= kPagedMaxRows, "paged_scratch_bytes");
+  static_assert(kSharedHeads || kWarps * Policy::kRows * kPitch <= static_cast<int>(kPagedHeadFloats),
+                "kPagedHeadFloats");
 };
 
 // Copies are made by the TMA unit, or by the lanes (kTma false).
@@ -99,6 +104,11 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   unsigned char* const rings = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<std::uintptr_t>(shared) + 1023) & ~static_cast<std::uintptr_t>(1023));
   unsigned char* const ring = rings + warp * S::kBytes;
+  const auto heads = [&] {
+    return S::kSharedHeads
+               ? reinterpret_cast<float*>(rings + kWarps * (S::kBytes + Policy::kWarpShared))
+               : a.aside + blockIdx.x * kPagedHeadFloats;
+  };
   if constexpr (kTma) {
     if (lane == 0) {
 #pragma unroll
@@ -331,10 +341,10 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     }
 
     // The segment ends.  A part goes to the ring, which is empty, when the warp
-    // is done, else out of its way.
+    // is done, else aside.
     const PagedUnit unit = paged_unit<kRows>(a, out.unit);
     const bool whole = begin == 0 && out.tile + 1 == out.tiles;
-    const bool spilled = to_read > 0;
+    const bool aside = to_read > 0;
     const int kind = begin == 0 ? kTail : kHead;
     if constexpr (!kTma) {
       if (!whole) copy_wait<0>();
@@ -344,13 +354,11 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       policy.finish_whole(a, unit, out.sequence, out.length == 0);
     else
       policy.finish_part(a, unit,
-                         spilled ? a.spill + range * a.row_cap * a.head_dim
-                                 : reinterpret_cast<float*>(ring),
-                         spilled ? a.head_dim : S::kPitch, parts.m[warp][kind],
-                         parts.l[warp][kind]);
+                         aside ? heads() + warp * kRows * S::kPitch : reinterpret_cast<float*>(ring),
+                         S::kPitch, parts.m[warp][kind], parts.l[warp][kind]);
     if (!whole && lane == 0)
       parts.records[warp][kind] = PartRecord{out.sequence, out.unit,     out.tiles, begin,
-                                             out.tile + 1, opens && kind == kHead, spilled};
+                                             out.tile + 1, opens && kind == kHead, aside};
     if (to_read > 0) {
       advance(out);
       begin = 0;
@@ -360,7 +368,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   if (reported != 0) watchdog_trip(a.watchdog, reported);
   __syncthreads();
   paged_merge<T, kWarps, kRows, S::kBytes / 4, S::kPitch, 4>(
-      a, parts, reinterpret_cast<const float*>(rings));
+      a, parts, reinterpret_cast<const float*>(rings), heads());
 }
 
 // Encodes a cache for the TMA unit; false when its layout does not allow it.
@@ -430,7 +438,7 @@ int paged_stream(PagedArgs a, cudaStream_t stream) {
   constexpr int kTile = Policy::kTile, kWidth = 128 / static_cast<int>(sizeof(T));
   if (a.pages > 0x7fffffff) a.pages = 0x7fffffff;  // as far as block-table entries reach
   const int grid = paged_grid(a, sm_count(), kTile, kWarps, Policy::kRows);
-  paged_scratch(&a, grid, kWarps, Policy::kRows);
+  paged_scratch(&a, grid, Policy::kRows);
   CUtensorMap k_map = {}, v_map = {};
   constexpr int kPieces = Policy::kDim / kWidth;
   MapOrder order = {a.page_size.divisor % kTile == 0 ? 1 : kTile / 8, kPieces};
