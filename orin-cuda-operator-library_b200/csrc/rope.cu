@@ -379,9 +379,10 @@ int kv_append(const void* q, int64_t q_token, int64_t q_head, const void* k, int
               int64_t out_token, int64_t out_head, const opl_kv_cache* cache, const int64_t* slots,
               int tokens, int heads, const opl_rope_spec* spec, cudaStream_t stream) {
   if (q == nullptr || k == nullptr || v == nullptr || q_out == nullptr || cache == nullptr ||
-      cache->k == nullptr || cache->v == nullptr || slots == nullptr || tokens <= 0 || heads <= 0 ||
-      cache->pages <= 0 || cache->page_size <= 0 || cache->kv_heads <= 0 || cache->head_dim <= 0 ||
-      cache->head_dim > kMaxHeadDim || !valid_rope(spec, cache->head_dim))
+      cache->k == nullptr || cache->v == nullptr || cache->k == cache->v || slots == nullptr ||
+      tokens <= 0 || heads <= 0 || cache->pages <= 0 || cache->page_size <= 0 ||
+      cache->kv_heads <= 0 || cache->head_dim <= 0 || cache->head_dim > kMaxHeadDim ||
+      !valid_rope(spec, cache->head_dim))
     return cudaErrorInvalidValue;
   RopeArgs<T> a = {};
   a.q = static_cast<const T*>(q);

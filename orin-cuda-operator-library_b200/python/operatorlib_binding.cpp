@@ -358,6 +358,7 @@ Tensor op_kv_append(const Tensor& q, const Tensor& k, const Tensor& v, Tensor& k
   TORCH_CHECK(k.size(1) == cache.kv_heads, "k and v must have the caches' key-value heads");
   require_no_overlap(k_cache, "k_cache");
   require_no_overlap(v_cache, "v_cache");
+  TORCH_CHECK(g_meta_call || cache.k != cache.v, "k_cache and v_cache must not share memory");
   require_cuda_contiguous(slots, "slots");
   require_type(slots, q, at::kLong, "slots", "int64");
   TORCH_CHECK(slots.dim() == 1 && slots.size(0) == tokens, "slots must have one element a token");

@@ -44,7 +44,7 @@ def rope_spec(**kw):
 
 
 def cache(**kw):
-    c = operatorlib.KvCache(FAKE, FAKE, 4, 16, 2, 64, 2048, 128, 64, 2048, 128, 64)
+    c = operatorlib.KvCache(FAKE, FAKE + 65536, 4, 16, 2, 64, 2048, 128, 64, 2048, 128, 64)
     for name, value in kw.items():
         setattr(c, name, value)
     return ctypes.byref(c)
@@ -74,7 +74,7 @@ def test_rope_refusals(suffix, change):
     dict(tokens=0), dict(heads=0), dict(cache=None), dict(cache=dict(k=None)),
     dict(cache=dict(v=None)), dict(cache=dict(pages=0)), dict(cache=dict(page_size=0)),
     dict(cache=dict(kv_heads=0)), dict(cache=dict(head_dim=0)), dict(cache=dict(head_dim=260)),
-    dict(cache=dict(head_dim=62)), dict(spec=dict(sections=[30])),
+    dict(cache=dict(head_dim=62)), dict(cache=dict(v=FAKE)), dict(spec=dict(sections=[30])),
 ])
 def test_kv_append_refusals(suffix, change):
     a = dict(q=FAKE, k=FAKE, v=FAKE, q_out=FAKE, slots=FAKE, tokens=3, heads=4, cache={}, spec={})

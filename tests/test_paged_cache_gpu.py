@@ -307,6 +307,15 @@ def test_kv_append_bad_slot_is_reported(ops):
     assert not v_cache.view(8, 64)[:7].any() and not k_cache.view(8, 64)[:7].any()
 
 
+def test_kv_append_refuses_one_cache_for_both(ops):
+    cache = torch.zeros(2, 4, 1, 64, device="cuda")
+    kv = randn(gen(3), 3, 1, 64)
+    index = torch.arange(3, device="cuda")
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        ops.kv_append(kv, kv, kv, cache, cache, index, index, torch.ones(32, device="cuda"))
+    assert not cache.any()
+
+
 # ----------------------------------------------------------- paged_attention
 
 @pytest.mark.parametrize("dtype", TYPES, ids=names)
