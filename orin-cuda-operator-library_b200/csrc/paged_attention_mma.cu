@@ -21,10 +21,13 @@
 //   in this lane -- and one byte permute a register pairs them; instruction e
 //   of 8 then computes columns 8n + e of the box, which lands 8 consecutive
 //   columns of a row in one lane.
-// * The weights enter P V as the sum of two 16-bit values, so that their
-//   rounding (2^-9 in BF16, as much as the result's own) does not show.  With
-//   up to 8 query heads a unit the second value rides in the 8 rows of the
-//   operand that are otherwise empty.
+// * The weights enter P V as the sum of two 16-bit values: one alone would
+//   round by 2^-8 in BF16, as much as the result itself; two leave 2^-16 of a
+//   weight, and 2^-22 in FP16.  FP16 also ends at steps of 2^-24, so its weights
+//   (and their sum: the factor cancels) are held times 2^15: half a step is
+//   2^-40 of the largest weight, not 2^-25, which a long tail below one key
+//   shows.  With up to 8 query heads a unit the second value rides in the 8
+//   rows of the operand that are otherwise empty.
 //
 // Running maximum, sum and output are FP32 in registers.
 #include "paged_stream.cuh"
@@ -37,6 +40,7 @@ template <typename T>
 struct Mma;
 template <>
 struct Mma<__half> {
+  static constexpr float kWeightScale = 32768.0f;  // of weights up to 1: all below 65504
   static __device__ __forceinline__ void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                              uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -56,6 +60,7 @@ struct Mma<__half> {
 };
 template <>
 struct Mma<__nv_bfloat16> {
+  static constexpr float kWeightScale = 1.0f;
   static __device__ __forceinline__ void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                              uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -96,7 +101,7 @@ struct MmaPolicy {
   using Query = uint4[kDim / 32][kHalves];
   Query qa, q_next;
   float o[kDim / 8][4];
-  float m[kHalves], l[kHalves];  // l over this lane's keys only
+  float m[kHalves], l[kHalves];  // l over this lane's keys only, times kWeightScale as o is
   int g, t;
   uint32_t k_piece, v_piece;  // where this lane's pieces lie
 
@@ -202,8 +207,8 @@ struct MmaPolicy {
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
-        const float x = paged_exp2(s[n][2 * h] - base[h]);
-        const float y = paged_exp2(s[n][2 * h + 1] - base[h]);
+        const float x = paged_exp2(s[n][2 * h] - base[h]) * Mma<T>::kWeightScale;
+        const float y = paged_exp2(s[n][2 * h + 1] - base[h]) * Mma<T>::kWeightScale;
         l[h] += x + y;
         p[n][h] = Mma<T>::split(x, y, &rest[n][h]);
       }

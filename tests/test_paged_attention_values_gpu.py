@@ -1,0 +1,68 @@
+"""Paged decode attention where single weights, values or pages are extreme: a
+key far above long tails of others, infinite and NaN values, sequences without
+any key in the cache.
+
+Tolerance of the tails, with u = 2^-24, n keys and head size D: a weight is off
+by the factor 2 (D + 6) u S_max (its score: D products, scaled; S_max the
+largest sum of their sizes) and 2^-22 (ex2.approx), numerator and denominator
+each, and their sums round by (n + 16) u each: with A = sum p_j |V_j|,
+A (4 (D + 6) u S_max + 2 (n + 16) u + 2^-20).  16-bit kernels hold a weight as
+two values of the type, 2^-16 relative.  In FP16 the second one's step ends at
+2^-24, of weights that are scaled so that the largest is 2^15: half a step is
+2^-40 of the largest weight, 2^-40 sum |V_j| / sum w with sum w >= 1.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from test_paged_cache_gpu import (TYPES, U, Paged, clean_watchdog, close, gen,  # noqa: F401
+                                  names, randn, watchdog)
+
+pytestmark = pytest.mark.gpu
+HALF_TYPES = [torch.float16, torch.bfloat16]
+
+
+# ------------------------------------------------------------- long tails
+
+def sink_inputs(dtype, heads, kv_heads, dim, batch, tail, gap, seed, sink):
+    """`batch` sequences over the same pages: key `sink` scores `gap` above the
+    `tail` others (all zero), and its value is 0."""
+    g = gen(seed)
+    page = 64
+    n = tail + 1
+    pages = -(-n // page)
+    k = torch.zeros(pages, page, kv_heads, dim, dtype=dtype, device="cuda")
+    v = (torch.rand(pages, page, kv_heads, dim, generator=g, device="cuda") + 0.5).to(dtype)
+    k[sink // page, sink % page, :, 0] = gap
+    v[sink // page, sink % page] = 0
+    q = randn(g, batch, heads, dim, dtype=dtype)
+    q[:, :, 0] = 1
+    table = torch.arange(pages, device="cuda", dtype=torch.int32).repeat(batch, 1)
+    lens = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    return q, k, v, table, lens
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("gap", [12.0, 17.0, 17.25, 17.375, 18.0, 20.0, 22.0])
+@pytest.mark.parametrize("heads,kv_heads,dim,batch,tail,sink", [
+    (4, 4, 64, 450, 8192, 0), (4, 4, 64, 450, 8192, 4100), (16, 1, 128, 1200, 4096, 0),
+    (6, 1, 80, 1, 131070, 7), (12, 1, 256, 3, 20000, 0), (4, 2, 71, 2, 5000, 60)])
+def test_tail_far_below_one_key(ops, dtype, gap, heads, kv_heads, dim, batch, tail, sink):
+    """Many keys far below one whose value is 0: the tail is the result.  With
+    many sequences a warp holds a whole one, with few it is cut."""
+    q, k, v, table, lens = sink_inputs(dtype, heads, kv_heads, dim, batch, tail, gap, dim, sink)
+    got = ops.paged_attention(q, k, v, table, lens, 1.0)
+    n = tail + 1
+    values = v.reshape(-1, kv_heads, dim)[:n].double()
+    weight = math.exp(-float(k[sink // 64, sink % 64, 0, 0]))
+    total = 1 + tail * weight
+    want = (values.sum(0) * weight / total).repeat_interleave(heads // kv_heads, 0)
+    slack = want * (4 * (dim + 6) * U * gap + 2 * (n + 16) * U + 2.0 ** -20)
+    if dtype != torch.float32:
+        slack = slack + 2.0 ** -16 * want
+    if dtype == torch.float16:
+        slack = slack + 2.0 ** -40 * values.sum(0).repeat_interleave(heads // kv_heads, 0) / total
+    close(got, want.expand_as(got), slack)
