@@ -58,6 +58,7 @@ struct FmaPolicy {
   static constexpr int kPieceBytes = kTile * 128;       // 32 columns of all keys
   static constexpr int kLanePieces = kDim / 32 / kSplit;
   static constexpr int kPairs = kDim / 64;              // column pairs of a lane
+  static constexpr bool kInfiniteValues = false;        // FP32 weights need no second look
   static constexpr int kQueryBytes = kRows * kDim * 4;
   static constexpr int kWarpShared = kQueryBytes + kRows * kTile * 8;  // and the weights
 
@@ -209,16 +210,17 @@ struct FmaPolicy {
       add_values<false>(values, seen);
   }
 
-  __device__ __forceinline__ void complete() {  // sums over the lanes of different keys
+  // Sums over the lanes of different keys.
+  __device__ __forceinline__ bool settle() {
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
 #pragma unroll
       for (int b = kSplit; b < 32; b <<= 1) l[r] += __shfl_xor_sync(kFullMask, l[r], b);
+    return false;
   }
 
   __device__ __forceinline__ void finish_whole(const PagedArgs& a, const PagedUnit& unit, int sequence,
                                                bool empty) {
-    complete();
     float* const dst = static_cast<float*>(a.out) +
                        (static_cast<int64_t>(sequence) * a.heads + unit.first_head) * a.head_dim;
 #pragma unroll
@@ -236,7 +238,6 @@ struct FmaPolicy {
 
   __device__ __forceinline__ void finish_part(const PagedArgs& a, const PagedUnit& unit, float* part,
                                               int pitch, float* part_m, float* part_l) {
-    complete();
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       if (r >= unit.rows) continue;
@@ -266,6 +267,7 @@ struct FmaRowsPolicy {
   static constexpr int kPieceBytes = kTile * 128;       // 32 columns of all keys
   static constexpr int kChunks = kDim / 32;             // 16-byte pieces of a lane
   static constexpr int kPairs = kDim / 64;              // column pairs of a lane
+  static constexpr bool kInfiniteValues = false;        // FP32 weights need no second look
   static constexpr int kQueryBytes = kRows * kDim * 4;
   static constexpr int kWarpShared = kQueryBytes + kRows * kTile * 4;  // and the weights
 
@@ -441,14 +443,15 @@ struct FmaRowsPolicy {
       add_values<false>(values, seen);
   }
 
-  __device__ __forceinline__ void complete() {  // sums over the groups
+  // Sums over the groups.
+  __device__ __forceinline__ bool settle() {
     l += __shfl_xor_sync(kFullMask, l, 8);
     l += __shfl_xor_sync(kFullMask, l, 16);
+    return false;
   }
 
   __device__ __forceinline__ void finish_whole(const PagedArgs& a, const PagedUnit& unit, int sequence,
                                                bool empty) {
-    complete();
     float* const dst = static_cast<float*>(a.out) +
                        (static_cast<int64_t>(sequence) * a.heads + unit.first_head) * a.head_dim;
     const float f = empty ? 0.0f : 1.0f / l;
@@ -468,7 +471,6 @@ struct FmaRowsPolicy {
 
   __device__ __forceinline__ void finish_part(const PagedArgs& a, const PagedUnit& unit, float* part,
                                               int pitch, float* part_m, float* part_l) {
-    complete();
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       if (r >= unit.rows) continue;

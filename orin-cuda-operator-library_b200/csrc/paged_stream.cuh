@@ -350,12 +350,28 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       if (!whole) copy_wait<0>();
     }
     __syncwarp();  // every lane has read its last stage
+    const bool odd = policy.settle();
+    const auto part = [&] {
+      return aside ? heads() + warp * kRows * S::kPitch : reinterpret_cast<float*>(ring);
+    };
     if (whole)
       policy.finish_whole(a, unit, out.sequence, out.length == 0);
     else
-      policy.finish_part(a, unit,
-                         aside ? heads() + warp * kRows * S::kPitch : reinterpret_cast<float*>(ring),
-                         S::kPitch, parts.m[warp][kind], parts.l[warp][kind]);
+      policy.finish_part(a, unit, part(), S::kPitch, parts.m[warp][kind], parts.l[warp][kind]);
+    if constexpr (Policy::kInfiniteValues) {
+      if (odd)
+        policy.infinite_values(
+            a, unit, out.sequence, begin * kTile, min(out.length, (out.tile + 1) * kTile),
+            [&](int row, int column, float x) {
+              if (whole)
+                st_out(static_cast<T*>(a.out) +
+                           (static_cast<int64_t>(out.sequence) * a.heads + unit.first_head + row) *
+                               a.head_dim + column,
+                       x);
+              else
+                part()[row * S::kPitch + column] = x;
+            });
+    }
     if (!whole && lane == 0)
       parts.records[warp][kind] = PartRecord{out.sequence, out.unit,     out.tiles, begin,
                                              out.tile + 1, opens && kind == kHead, aside};

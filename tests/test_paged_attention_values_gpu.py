@@ -66,3 +66,50 @@ def test_tail_far_below_one_key(ops, dtype, gap, heads, kv_heads, dim, batch, ta
     if dtype == torch.float16:
         slack = slack + 2.0 ** -40 * values.sum(0).repeat_interleave(heads // kv_heads, 0) / total
     close(got, want.expand_as(got), slack)
+
+
+# ------------------------------------------------- infinite and NaN values
+
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("heads", [2, 12, 16, 32])
+@pytest.mark.parametrize("dim", [64, 80, 128, 192, 256, 71])
+@pytest.mark.parametrize("lens", [[100, 40], [3000, 70], [100] * 900], ids=lambda x: f"{len(x)}x{x[0]}")
+def test_infinite_values(ops, dtype, heads, dim, lens):
+    """Column d of key-value head 1 reads an infinity from key d (weights of
+    all sizes): infinite, with its sign; NaN where both signs or a NaN are
+    read; and nothing else changes."""
+    cache = Paged(lens, 2, dim, 16, dtype, 25)
+    q = randn(gen(1), len(lens), heads, dim, dtype=dtype)
+    clean = ops.paged_attention(q, cache.k, cache.v, cache.table, cache.seq_lens)
+    v = cache.v.clone()
+
+    def put(key, column, value):
+        v[cache.table[0, key // 16].long(), key % 16, 1, column] = value
+
+    want = clean.clone()
+    for column in range(0, dim - 8, 2):
+        sign = 1 if column % 4 else -1
+        put(column % 100, column, sign * math.inf)
+        want[0, heads // 2:, column] = sign * math.inf
+    for column, values in ((dim - 1, (math.inf, -math.inf)), (dim - 3, (math.nan,)),
+                           (dim - 5, (math.inf, math.nan)), (dim - 7, (-math.inf, -math.inf))):
+        for key, value in zip((3, 90), values):
+            put(key, column, value)
+        want[0, heads // 2:, column] = math.nan if dim - column < 7 else -math.inf
+    got = ops.paged_attention(q, cache.k, v, cache.table, cache.seq_lens)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("heads", [1, 8, 16])
+@pytest.mark.parametrize("gap", [8.0, 16.0, 24.0, 40.0, 80.0])
+def test_infinite_value_of_small_weight(ops, dtype, heads, gap):
+    """An infinity counts as long as FP32 holds its weight (e^-87)."""
+    q, k, v, table, lens = sink_inputs(dtype, heads, 1, 64, 3, 500, gap, 3, 200)
+    v[1, 7, 0, 11] = math.inf
+    v[5, 7, 0, 12] = -math.inf
+    got = ops.paged_attention(q, k, v, table, lens, 1.0)
+    assert (got[..., 11] == math.inf).all() and (got[..., 12] == -math.inf).all()
+    got[..., 11:13] = 0
+    assert got.isfinite().all()
