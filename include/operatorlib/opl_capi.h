@@ -217,11 +217,11 @@ int opl_kv_append_bf16(const opl_bf16_t* q, int64_t q_token, int64_t q_head, con
  * head_dim] (out contiguous, overlapping nothing), query head h reads key-value head
  * h / (heads / kv_heads), and sequence b has seq_lens[b] keys, key j in page
  * block_table[b * table_row + j / page_size].  Softmax over scale * q.K in
- * FP32; the result is rounded once to the tensors' type.  A sequence of length
- * 0 gives zeros.  Table entries past a sequence's pages are not read, and
- * neither are a page's tokens past its length.  Keys of a page outside the
- * cache are left out.  max_pages * page_size is at most 2^30, and batch times
- * that at most 2^34.
+ * FP32; the result is rounded once to the tensors' type.  Keys of a page outside
+ * the cache are left out.  A sequence without keys (of length 0, or with all of
+ * its pages outside) gives zeros.  Table entries past a sequence's pages are not
+ * read, and neither are a page's tokens past its length.  max_pages * page_size is
+ * at most 2^30, and batch times that at most 2^34.
  * `workspace` is 16-byte aligned device memory of at least the size that
  * opl_paged_attention_workspace gives; its contents do not matter and need not
  * be kept, but two calls that may overlap on the GPU need one each. */

@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
       for (int e = 0; e < E; ++e) o[r][e] = 0.0f;
     }
     float m = -INFINITY, l = 0.0f;  // of my_row; l over my keys only
+    bool has_keys = false;
 
     for (int tile = at.tile; tile < end; ++tile) {
       const int base = tile * kTile;
@@ -168,6 +169,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
             reported = kBadPage;
         }
       }
+      has_keys |= __any_sync(kFullMask, place >= 0);
       float kr[kTile][E], vr[kTile][E];
 #pragma unroll
       for (int j = 0; j < kTile; ++j) {
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const int d = lane + 32 * e;
-          if (d < a.head_dim) st_out(dst + d, length == 0 ? 0.0f : o[r][e] / sum);
+          if (d < a.head_dim) st_out(dst + d, has_keys ? o[r][e] / sum : 0.0f);
         }
       }
       continue;
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
     const bool aside = w < limit;
     float* const part = (aside ? heads : rows) + warp * kRows * kWidth;
     if (lane % kLanesOfRow == 0 && my_row < unit.rows) {
-      parts.m[warp][kind][my_row] = m;
+      parts.m[warp][kind][my_row] = fmaxf(m, least_maximum(has_keys));
       parts.l[warp][kind][my_row] = l;
     }
 #pragma unroll

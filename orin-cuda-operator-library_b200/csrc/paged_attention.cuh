@@ -219,6 +219,24 @@ __device__ __forceinline__ void ld_row_l2(const float* p, float (&x)[kWidth]) {
   }
 }
 
+// The least maximum of a part.  A part without keys (of pages outside the cache)
+// has -infinity, and where all parts of a unit have, the result is zero.  One
+// whose keys all score -infinity has the lowest number, so that nothing but such
+// parts gives 0 / 0, as the formula does.
+__device__ __forceinline__ float least_maximum(bool keys) {
+  return keys ? -3.402823466e38f : -INFINITY;
+}
+
+// Whether any of a sequence's keys first .. end - 1 lies in the cache.
+__device__ __forceinline__ bool any_page(const PagedArgs& a, int sequence, int first, int end) {
+  bool found = false;
+#pragma unroll 1
+  for (int key = first + (threadIdx.x & 31); key < end && !found; key += 32)
+    found = cache_page(ld_int(a.block_table + sequence * a.table_row + fast_div(key, a.page_size)),
+                       a.pages);
+  return __any_sync(kFullMask, found);
+}
+
 // What the warps of a CTA leave for one another in shared memory.
 template <int kWarps, int kRows>
 struct PagedParts {
@@ -314,9 +332,11 @@ __device__ __forceinline__ void paged_merge(const PagedArgs& a, PagedParts<kWarp
           const int at = row + q * step;
           if (at >= unit.rows) continue;
           const float sum = parts.sum[start >> 1][start & 1][at];
+          const bool none = parts.top[start >> 1][start & 1][at] == -INFINITY;  // no key
           if (whole) {
 #pragma unroll
-            for (int e = 0; e < kWidth; ++e) out[q][e] = __fdividef(out[q][e], sum);
+            for (int e = 0; e < kWidth; ++e)
+              out[q][e] = none ? 0.0f : __fdividef(out[q][e], sum);
             st_row(static_cast<T*>(a.out) +
                        (static_cast<int64_t>(r.sequence) * a.heads + unit.first_head + at) * a.head_dim +
                        d,
@@ -423,7 +443,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
     for (int w = 0; w < kJoinWarps; ++w) l += warp_sum[w], o += rows[w][d];
     st_out(static_cast<T*>(a.out) +
                (static_cast<int64_t>(sequence) * a.heads + unit.first_head + row) * a.head_dim + d,
-           __fdividef(o, l));
+           top == -INFINITY ? 0.0f : __fdividef(o, l));
   }
 }
 

@@ -358,19 +358,24 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       policy.finish_whole(a, unit, out.sequence, out.length == 0);
     else
       policy.finish_part(a, unit, part(), S::kPitch, parts.m[warp][kind], parts.l[warp][kind]);
-    if constexpr (Policy::kInfiniteValues) {
-      if (odd)
-        policy.infinite_values(
-            a, unit, out.sequence, begin * kTile, min(out.length, (out.tile + 1) * kTile),
-            [&](int row, int column, float x) {
-              if (whole)
-                st_out(static_cast<T*>(a.out) +
-                           (static_cast<int64_t>(out.sequence) * a.heads + unit.first_head + row) *
-                               a.head_dim + column,
-                       x);
-              else
-                part()[row * S::kPitch + column] = x;
-            });
+    if (odd && out.length != 0) {
+      const int first = begin * kTile, end = min(out.length, (out.tile + 1) * kTile);
+      T* const rows = static_cast<T*>(a.out) +
+                      (static_cast<int64_t>(out.sequence) * a.heads + unit.first_head) * a.head_dim;
+      if constexpr (Policy::kInfiniteValues)
+        policy.infinite_values(a, unit, out.sequence, first, end, [&](int row, int column, float x) {
+          if (whole)
+            st_out(rows + row * a.head_dim + column, x);
+          else
+            part()[row * S::kPitch + column] = x;
+        });
+      const bool keys = any_page(a, out.sequence, first, end);
+      __syncwarp();  // what the other lanes have written
+      if (whole && !keys) {
+        for (int i = lane; i < unit.rows * a.head_dim; i += 32) st_out(rows + i, 0.0f);
+      } else if (!whole && lane < unit.rows) {
+        parts.m[warp][kind][lane] = fmaxf(parts.m[warp][kind][lane], least_maximum(keys));
+      }
     }
     if (!whole && lane == 0)
       parts.records[warp][kind] = PartRecord{out.sequence, out.unit,     out.tiles, begin,

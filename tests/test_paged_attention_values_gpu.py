@@ -113,3 +113,45 @@ def test_infinite_value_of_small_weight(ops, dtype, heads, gap):
     assert (got[..., 11] == math.inf).all() and (got[..., 12] == -math.inf).all()
     got[..., 11:13] = 0
     assert got.isfinite().all()
+
+
+# ------------------------------------------------------ no key in the cache
+
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("heads", [2, 12, 32])
+@pytest.mark.parametrize("dim", [64, 128, 256, 71])
+@pytest.mark.parametrize("lens", [[40, 30], [6000, 70], [20] * 900], ids=lambda x: f"{len(x)}x{x[0]}")
+def test_sequence_with_every_page_outside(ops, dtype, heads, dim, lens):
+    """Its keys are left out, so it has none and gives zeros, whether one warp
+    holds it or it is cut over many CTAs; the others keep their bits."""
+    cache = Paged(lens, 2, dim, 16, dtype, 27)
+    q = randn(gen(1), len(lens), heads, dim, dtype=dtype)
+    clean = ops.paged_attention(q, cache.k, cache.v, cache.table, cache.seq_lens)
+    table = cache.table.clone()
+    table[0] = cache.k.shape[0]
+    got = ops.paged_attention(q, cache.k, cache.v, table, cache.seq_lens)
+    assert watchdog() == 0x6b02
+    assert not got[0].any() and torch.equal(got[1:], clean[1:])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("heads", [2, 12, 32])
+@pytest.mark.parametrize("dim", [64, 256, 71])
+@pytest.mark.parametrize("n", [40, 6000])
+def test_scores_all_minus_infinity(ops, dtype, heads, dim, n):
+    """Keys that all score -inf are keys: 0 / 0, as the formula has it.  One
+    finite score among them, or in another part of the sequence, is the
+    result."""
+    cache = Paged([n, 9], 2, dim, 16, dtype, 28)
+    q = randn(gen(1), 2, heads, dim, dtype=dtype).abs()
+    clean = ops.paged_attention(q, cache.k, cache.v, cache.table, cache.seq_lens)
+    k = cache.k.clone()
+    k[cache.table[0].long()] = -math.inf
+    got = ops.paged_attention(q, k, cache.v, cache.table, cache.seq_lens)
+    assert got[0].isnan().all() and torch.equal(got[1], clean[1])
+    key = n - 3
+    page = cache.table[0, key // 16].long()
+    k[page, key % 16] = 0
+    got = ops.paged_attention(q, k, cache.v, cache.table, cache.seq_lens)
+    want = cache.v[page, key % 16].repeat_interleave(heads // 2, 0)
+    assert torch.equal(got[0], want) and torch.equal(got[1], clean[1])
