@@ -210,14 +210,15 @@ struct FmaPolicy {
       add_values<false>(values, seen);
   }
 
-  // Sums over the lanes of different keys.  True when no key has a weight.
+  // Sums over the lanes of different keys.  True when no key has a weight, or a
+  // score is no number.
   __device__ __forceinline__ bool settle() {
     bool none = false;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
 #pragma unroll
       for (int b = kSplit; b < 32; b <<= 1) l[r] += __shfl_xor_sync(kFullMask, l[r], b);
-      none |= l[r] == 0.0f;  // in all lanes
+      none |= !(l[r] > 0.0f);  // in all lanes
     }
     return none;
   }
@@ -446,11 +447,12 @@ struct FmaRowsPolicy {
       add_values<false>(values, seen);
   }
 
-  // Sums over the groups.  True when no key has a weight.
+  // Sums over the groups.  True when no key has a weight, or a
+  // score is no number.
   __device__ __forceinline__ bool settle() {
     l += __shfl_xor_sync(kFullMask, l, 8);
     l += __shfl_xor_sync(kFullMask, l, 16);
-    return __any_sync(kFullMask, l == 0.0f);
+    return __any_sync(kFullMask, !(l > 0.0f));
   }
 
   __device__ __forceinline__ void finish_whole(const PagedArgs& a, const PagedUnit& unit, int sequence,

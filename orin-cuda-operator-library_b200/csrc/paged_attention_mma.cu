@@ -250,7 +250,8 @@ struct MmaPolicy {
   }
 
   // Ends a segment: sums over the lanes that hold different keys.  True when an
-  // output is not finite (see infinite_values) or no key has a weight.
+  // output is not finite (see infinite_values), no key has a weight, or a score is no
+  // number.
   __device__ __forceinline__ bool settle() {
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
@@ -268,7 +269,7 @@ struct MmaPolicy {
         odd[2 * (n & 1) + x] = fmaf(o[n][x], 0.0f, odd[2 * (n & 1) + x]);
       }
     const float any = (odd[0] + odd[1]) + (odd[2] + odd[3]);
-    return __any_sync(kFullMask, any != any || l[0] == 0.0f || l[kHalves - 1] == 0.0f);
+    return __any_sync(kFullMask, any != any || !(l[0] > 0.0f) || !(l[kHalves - 1] > 0.0f));
   }
 
   // An infinite value times the two parts of a weight, of which the second may

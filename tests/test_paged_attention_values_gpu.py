@@ -155,3 +155,25 @@ def test_scores_all_minus_infinity(ops, dtype, heads, dim, n):
     got = ops.paged_attention(q, k, cache.v, cache.table, cache.seq_lens)
     want = cache.v[page, key % 16].repeat_interleave(heads // 2, 0)
     assert torch.equal(got[0], want) and torch.equal(got[1], clean[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=names)
+@pytest.mark.parametrize("heads", [2, 12, 32])
+@pytest.mark.parametrize("dim", [64, 256, 71])
+@pytest.mark.parametrize("n", [40, 6000])
+def test_scores_all_nan(ops, dtype, heads, dim, n):
+    """A query or keys that are no numbers: neither is the result, whole or cut."""
+    cache = Paged([n, 9], 2, dim, 16, dtype, 29)
+    q = randn(gen(1), 2, heads, dim, dtype=dtype)
+    clean = ops.paged_attention(q, cache.k, cache.v, cache.table, cache.seq_lens)
+    bad = q.clone()
+    bad[0, 0] = math.nan
+    got = ops.paged_attention(bad, cache.k, cache.v, cache.table, cache.seq_lens)
+    assert got[0, 0].isnan().all()
+    assert torch.equal(got[0, 1:], clean[0, 1:]) and torch.equal(got[1], clean[1])
+    k = cache.k.clone()
+    k[cache.table[0].long(), :, 1] = math.nan
+    got = ops.paged_attention(q, k, cache.v, cache.table, cache.seq_lens)
+    assert got[0, heads // 2:].isnan().all()
+    assert torch.equal(got[0, :heads // 2], clean[0, :heads // 2])
+    assert torch.equal(got[1], clean[1])
