@@ -5,7 +5,9 @@ outputs, passes their device pointers and the current CUDA stream (or
 ``stream``) to the matching ``opl_*`` entry point and raises ``OplError`` on a
 non-zero return -- the same contract a C, cgo or JNI caller gets.  The paged
 cache functions (``rope_into``, ``kv_append_into``, ``paged_attention_into``)
-take strided tensors whose last dimension is contiguous.
+take strided tensors whose last dimension is contiguous, and raise ``ValueError``
+for operands whose shapes, types or devices do not go together: the C entries
+see pointers only and would read or write past them.
 """
 from __future__ import annotations
 
@@ -90,13 +92,46 @@ def attention_into(q, k, v, out, causal: bool, stream=None) -> None:
                            int(bool(causal)), _stream(q, stream)))
 
 
-def _rope_spec(positions, inv_freq, sections, adjacent, inverse):
+def _require_rows(name, t, like, shape=None, written=False) -> None:
+    """A strided operand: like's dtype and device, the last dimension contiguous."""
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must have the other tensors' dtype and device")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have the shape {list(shape)}")
+    strides = t.stride()
+    if strides[-1] != 1 and t.shape[-1] != 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    if written and 0 in strides and any(s == 0 and n > 1 for s, n in zip(strides, t.shape)):
+        raise ValueError(f"{name} is written and must not be expanded")
+
+
+def _require_index(name, t, like, dtype, shape) -> None:
+    """Contiguous numbers that the kernel indexes by itself."""
+    if t.dtype != dtype or t.device != like.device:
+        raise ValueError(f"{name} must be {str(dtype).split('.')[-1]} on the other tensors' device")
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous with the shape {list(shape)}")
+
+
+def _require_dims(name, t, dims) -> None:
+    if t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions")
+
+
+def _rope_spec(x, positions, inv_freq, sections, adjacent, inverse):
+    import torch
+
     from . import RopeSpec
 
-    pairs = inv_freq.numel()
+    pairs, tokens = inv_freq.numel(), x.shape[0]
     sections = list(sections) if sections else [pairs]
     if len(sections) > 4:
         raise ValueError("a rotary embedding has at most 4 position axes")
+    _require_index("inv_freq", inv_freq, x, torch.float32, (pairs,))
+    # One axis may come as [tokens] or [1, tokens].
+    whole = len(sections) == 1 and positions.dim() == 1
+    _require_index("positions", positions, x, torch.int64,
+                   (tokens,) if whole else (len(sections), tokens))
     spec = RopeSpec(positions=_ptr(positions), inv_freq=_ptr(inv_freq), rot_dim=2 * pairs,
                     axes=len(sections), adjacent=int(bool(adjacent)),
                     inverse=int(bool(inverse)))
@@ -104,9 +139,15 @@ def _rope_spec(positions, inv_freq, sections, adjacent, inverse):
     return spec
 
 
-def _kv_cache(k_cache, v_cache):
+def _kv_cache(q, k_cache, v_cache, written):
     from . import KvCache
 
+    _require_dims("k_cache", k_cache, 4)
+    _require_rows("k_cache", k_cache, q, written=written)
+    _require_rows("v_cache", v_cache, q, k_cache.shape, written=written)
+    if k_cache.shape[3] != q.shape[2]:
+        raise ValueError("the caches must be [pages, page_size, kv_heads, head_dim] with q's "
+                         "head_dim")
     pages, page_size, kv_heads, head_dim = k_cache.shape
     return KvCache(_ptr(k_cache), _ptr(v_cache), pages, page_size, kv_heads, head_dim,
                    *k_cache.stride()[:3], *v_cache.stride()[:3])
@@ -121,8 +162,11 @@ def rope_into(x, out, positions, inv_freq, sections=None, adjacent=False, invers
 
     import torch
 
+    _require_dims("x", x, 3)
+    _require_rows("x", x, x)
+    _require_rows("out", out, x, x.shape, written=True)
     tokens, heads, head_dim = x.shape
-    spec = _rope_spec(positions, inv_freq, sections, adjacent, inverse)
+    spec = _rope_spec(x, positions, inv_freq, sections, adjacent, inverse)
     with torch.cuda.device(x.device):
         _check("rope", _dtype_fn("rope", x.dtype)(
             _ptr(x), _ptr(out), tokens, heads, head_dim, *x.stride()[:2], *out.stride()[:2],
@@ -139,8 +183,15 @@ def kv_append_into(q, k, v, q_out, k_cache, v_cache, slots, positions, inv_freq,
 
     import torch
 
-    spec = _rope_spec(positions, inv_freq, sections, adjacent, False)
-    cache = _kv_cache(k_cache, v_cache)
+    _require_dims("q", q, 3)
+    _require_rows("q", q, q)
+    _require_rows("q_out", q_out, q, q.shape, written=True)
+    cache = _kv_cache(q, k_cache, v_cache, written=True)
+    new = (q.shape[0], *k_cache.shape[2:])
+    _require_rows("k", k, q, new)
+    _require_rows("v", v, q, new)
+    _require_index("slots", slots, q, torch.int64, (q.shape[0],))
+    spec = _rope_spec(q, positions, inv_freq, sections, adjacent, False)
     with torch.cuda.device(q.device):
         _check("kv_append", _dtype_fn("kv_append", q.dtype)(
             _ptr(q), *q.stride()[:2], _ptr(k), *k.stride()[:2], _ptr(v), *v.stride()[:2],
@@ -171,12 +222,24 @@ def paged_attention_into(q, k_cache, v_cache, block_table, seq_lens, out, worksp
 
     import torch
 
+    _require_dims("q", q, 3)
+    _require_rows("q", q, q)
+    _require_index("out", out, q, q.dtype, q.shape)
+    cache = _kv_cache(q, k_cache, v_cache, written=False)
     batch, heads, head_dim = q.shape
-    cache = _kv_cache(k_cache, v_cache)
+    _require_dims("block_table", block_table, 2)
+    columns = block_table.shape[1]
+    if (block_table.dtype != torch.int32 or block_table.device != q.device
+            or block_table.shape[0] != batch or (block_table.stride(1) != 1 and columns != 1)):
+        raise ValueError("block_table must be int32 [batch, pages] on the other tensors' device, "
+                         "contiguous in its last dimension")
+    _require_index("seq_lens", seq_lens, q, torch.int32, (batch,))
+    if workspace.device != q.device or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous on the other tensors' device")
     scale = head_dim ** -0.5 if scale is None else float(scale)
     with torch.cuda.device(q.device):
         _check("paged_attention", _dtype_fn("paged_attention", q.dtype)(
             _ptr(q), *q.stride()[:2], ctypes.byref(cache), _ptr(block_table),
-            block_table.stride(0), block_table.shape[1], _ptr(seq_lens), _ptr(out), batch, heads,
+            block_table.stride(0), columns, _ptr(seq_lens), _ptr(out), batch, heads,
             scale, _ptr(workspace), workspace.numel() * workspace.element_size(),
             _stream(q, stream)))
