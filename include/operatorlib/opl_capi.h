@@ -220,8 +220,10 @@ int opl_kv_append_bf16(const opl_bf16_t* q, int64_t q_token, int64_t q_head, con
  * FP32; the result is rounded once to the tensors' type.  Keys of a page outside
  * the cache are left out.  A sequence without keys (of length 0, or with all of
  * its pages outside) gives zeros.  Table entries past a sequence's pages are not
- * read, and neither are a page's tokens past its length.  max_pages * page_size is
- * at most 2^30, and batch times that at most 2^34.
+ * read.  A page's tokens past its length may be fetched together with those in
+ * front of them, but what they hold, or what is being written there, does not
+ * matter.  max_pages * page_size is at most 2^30, and batch times that at most
+ * 2^34.
  * `workspace` is 16-byte aligned device memory of at least the size that
  * opl_paged_attention_workspace gives; its contents do not matter and need not
  * be kept, but two calls that may overlap on the GPU need one each. */
