@@ -293,9 +293,12 @@ int launch_rope(RopeArgs<T> a, int heads, int kv_heads, int head_dim, const opl_
   a.pair_items = a.rot_dim / 2 / vector;
   const int row_items = a.pair_items + (head_dim - a.rot_dim) / vector;
   const int v_row_items = head_dim / vector;
-  const int64_t items =
-      static_cast<int64_t>(heads + kv_heads) * row_items + static_cast<int64_t>(kv_heads) * v_row_items;
+  const int64_t items = (int64_t{heads} + kv_heads) * row_items + int64_t{kv_heads} * v_row_items;
   if (items > (int64_t{1} << 30)) return cudaErrorInvalidValue;
+  if (a.slots != nullptr) {
+    a.watchdog = watchdog_word();
+    if (a.watchdog == nullptr) return cudaErrorInvalidDevice;
+  }
   a.row_items = make_fast_div(row_items);
   a.v_row_items = make_fast_div(v_row_items);
   a.q_items = heads * row_items;
@@ -409,8 +412,6 @@ int kv_append(const void* q, int64_t q_token, int64_t q_head, const void* k, int
   a.pages = cache->pages;
   a.page_size = cache->page_size;
   a.tokens = tokens;
-  a.watchdog = watchdog_word();
-  if (a.watchdog == nullptr) return cudaErrorInvalidDevice;
   return launch_rope(a, heads, cache->kv_heads, cache->head_dim, spec, stream);
 }
 

@@ -3,6 +3,8 @@ the C entries see pointers only.  Without a GPU: every call is refused before
 a pointer is used."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -122,3 +124,18 @@ def test_operands_that_go_together_are_not_refused():
                            block_table=t(5, 9, dtype=I32)[:, 2:4]))):
         with pytest.raises(ValueError, match="Expected a cuda device"):
             call(**args)
+
+
+@pytest.mark.parametrize("suffix", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads", [(2 ** 31 - 1, 1), (2 ** 31 - 1, 2 ** 31 - 1),
+                                            (2 ** 30, 2 ** 30), (2 ** 27, 1)])
+def test_too_many_heads(suffix, heads, kv_heads):
+    """More than 2^30 vectors a token, counted in 64 bits: invalid argument."""
+    fake = 0x1000  # never dereferenced
+    spec = operatorlib.RopeSpec(fake, fake, 64, 1)
+    spec.sections[0] = 32
+    cache = operatorlib.KvCache(fake, fake + 65536, 4, 16, kv_heads, 64, 2048, 128, 64, 2048, 128,
+                                64)
+    fn = getattr(operatorlib.capi(), f"opl_kv_append_{suffix}")
+    assert fn(fake, 256, 1, fake, 128, 64, fake, 128, 64, fake, 256, 64, ctypes.byref(cache), fake,
+              3, heads, ctypes.byref(spec), None) == 1
