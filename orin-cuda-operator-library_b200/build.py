@@ -51,7 +51,7 @@ TORCH_LIB_NAME = "_operatorlib_torch.so"
 
 
 def _headers() -> list[Path]:
-    return sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.rglob("*.h"))
+    return sorted([*CSRC.glob("*.cuh"), *CSRC.glob("*.h"), *INCLUDE.rglob("*.h")])
 
 
 def _stale(target: Path, deps: list[Path]) -> bool:
