@@ -277,45 +277,64 @@ struct MmaPolicy {
   // infinity or NaN among keys first .. end - 1 of the segment are written again
   // from a second look at them: store(row, column, value).  After the outputs,
   // whose registers are free then (before them: 16/1 heads of 256 33.6 us).  The
-  // sums that call for it cost 0.8% of 256 short sequences, 31.0 -> 31.24 us, and
-  // 3% of 16/1 heads of 256, 31.4 -> 32.3 us.
+  // sums that call for it cost 1.5% of 256 short sequences, 31.0 -> 31.5 us, and
+  // 4% of 16/1 heads of 256, 31.4 -> 32.7 us.  The look itself, where it is taken:
+  // 314 -> 781 us for 128 sequences of up to 8191 keys, every value NaN.
   template <typename Store>
   __device__ __forceinline__ void infinite_values(const PagedArgs& a, const PagedUnit& unit,
                                                   int sequence, int first, int end,
                                                   Store store) const {
+    bool sums = false;  // a row with a sum; the others are no numbers at all
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) sums |= g + 8 * h < unit.rows && l[h] > 0.0f;
+    if (!__any_sync(kFullMask, sums)) return;
     const int* const table = a.block_table + sequence * a.table_row;
     const T* const head = static_cast<const T*>(a.v) + unit.kv_head * a.v_head;
+    // Pieces of 8 columns, as in each(): all at once, but one by one for heads over
+    // 128, whose kernels have no registers to spare (32.7 against 33.8 us).
+    constexpr int kPieces = kDim > 128 ? 1 : kDim / 32;
 #pragma unroll 1
-    for (int piece = 0; piece < kDim / 32; ++piece) {  // columns d .. d + 7
-      const int d = 64 * (piece / 2) + 16 * t + 8 * (piece & 1);
-      uint32_t signs = 0;  // bit e: column d + e reads an infinity; bit 8 + e: one below 0
+    for (int piece = 0; piece < kDim / 32; piece += kPieces) {
+      const auto column = [&](int i) {
+        return 64 * ((piece + i) / 2) + 16 * t + 8 * ((piece + i) & 1);
+      };
+      uint32_t signs[kPieces] = {};  // bit e: column e reads an infinity; 8 + e: one below 0
 #pragma unroll 1
-      for (int key = first + g; key < end && d < a.head_dim; key += 8) {
+      for (int key = first + g; key < end; key += 8) {
         const int row = static_cast<int>(fast_div(key, a.page_size));
         const int page = ld_int(table + row);
         if (!cache_page(page, a.pages)) continue;
         const int inside = key - row * static_cast<int>(a.page_size.divisor);
-        const uint4 v = ld_ro(
-            reinterpret_cast<const uint4*>(head + page * a.v_page + inside * a.v_token + d));
+        const T* const src = head + page * a.v_page + inside * a.v_token;
+        uint4 v[kPieces];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t bits = word(v, e / 2) >> (16 * (e & 1)) & 0xffffu;
-          const bool nan = (bits & 0x7fffu) > Mma<T>::kInfinity;  // as both infinities
-          if (nan || bits == Mma<T>::kInfinity) signs |= 1u << e;
-          if (nan || bits == (0x8000u | Mma<T>::kInfinity)) signs |= 0x100u << e;
-        }
+        for (int i = 0; i < kPieces; ++i)
+          v[i] = column(i) < a.head_dim ? ld_ro(reinterpret_cast<const uint4*>(src + column(i)))
+                                        : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t bits = word(v[i], e / 2) >> (16 * (e & 1)) & 0xffffu;
+            const bool nan = (bits & 0x7fffu) > Mma<T>::kInfinity;  // as both infinities
+            if (nan || bits == Mma<T>::kInfinity) signs[i] |= 1u << e;
+            if (nan || bits == (0x8000u | Mma<T>::kInfinity)) signs[i] |= 0x100u << e;
+          }
       }
       __syncwarp();
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) signs |= __shfl_xor_sync(kFullMask, signs, x);
+      for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const int row = g + 8 * h;
-        if (row >= unit.rows || !(l[h] > 0.0f)) continue;  // the others are no numbers at all
+        for (int x = 4; x < 32; x <<= 1) signs[i] |= __shfl_xor_sync(kFullMask, signs[i], x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t sign = signs >> e & 0x101u;
-          if (sign != 0) store(row, d + e, sign == 1 ? INFINITY : sign == 0x100 ? -INFINITY : NAN);
+        for (int h = 0; h < kHalves; ++h) {
+          if (g + 8 * h >= unit.rows || !(l[h] > 0.0f)) continue;
+#pragma unroll 1
+          for (uint32_t left = (signs[i] | signs[i] >> 8) & 0xffu; left != 0; left &= left - 1) {
+            const int e = __ffs(left) - 1;
+            const uint32_t sign = signs[i] >> e & 0x101u;
+            store(g + 8 * h, column(i) + e, sign == 1 ? INFINITY : sign == 0x100 ? -INFINITY : NAN);
+          }
         }
       }
     }
