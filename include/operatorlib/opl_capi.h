@@ -196,7 +196,8 @@ int opl_rope_bf16(const opl_bf16_t* x, opl_bf16_t* out, int tokens, int heads, i
  * negative have to be distinct: of two tokens with the same slot either may
  * win, element by element.  Nothing else of the cache is touched; its keys and
  * values share no memory.  q is [tokens, heads, head_dim]; k and v are
- * [tokens, kv_heads, head_dim]; q_out is q itself or overlaps nothing. */
+ * [tokens, kv_heads, head_dim]; none of them overlaps the cache (tokens are not
+ * moved within it by this call); q_out is q itself or overlaps nothing. */
 int opl_kv_append_f32(const float* q, int64_t q_token, int64_t q_head, const float* k,
                       int64_t k_token, int64_t k_head, const float* v, int64_t v_token,
                       int64_t v_head, float* q_out, int64_t out_token, int64_t out_head,

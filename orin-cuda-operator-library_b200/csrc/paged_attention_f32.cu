@@ -257,7 +257,7 @@ struct FmaPolicy {
 };
 
 // Eight rows, heads of up to 128 (11 sequences of 7098 keys, 64/4 heads of 128:
-// 122 us against 170 us for FmaPolicy; 97 are the reading of keys and values for
+// 123 us against 170 us for FmaPolicy; 97 are the reading of keys and values for
 // each of the two units of a head).  Reading Q for every key would keep shared
 // memory busy three times as long as the products take, so the 8 lanes of a key group share its keys' columns and
 // each takes 2 (heads of 64: 4) keys against one piece of Q; the transposing sum

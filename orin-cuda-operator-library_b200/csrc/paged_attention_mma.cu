@@ -394,7 +394,8 @@ template <typename T, int kRows>
 int pick_dim(const PagedArgs& a, cudaStream_t stream) {
   // Warps and stages by head size.  64: 12 x 2 at 168 registers (100,000 keys, 8
   // heads: 71 us; 8 x 3, 82 us; 16 x 2 the same as 12).  128: see
-  // paged_stream.cuh.  Over 128 four warps, for their registers.
+  // paged_stream.cuh.  Over 128 four warps of 32 to 36 KB of ring each, at 255
+  // registers; 16 rows of 256 spill (184 bytes stored).
   if (a.head_dim <= 64) return paged_stream<MmaPolicy<T, 64, kRows>, 12, 2>(a, stream);
   if (a.head_dim <= 128) return paged_stream<MmaPolicy<T, 128, kRows>, 8, 2>(a, stream);
   if (a.head_dim <= 192) return paged_stream<MmaPolicy<T, 192, kRows>, 4, 3>(a, stream);

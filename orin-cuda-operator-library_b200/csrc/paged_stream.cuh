@@ -14,7 +14,8 @@
 //   their issue alone bounds the kernel (106 us with no arithmetic, 138 us when
 //   a group of eight lanes does not cover 128 bytes of a row; TMA 87 us with it).
 // * Two stages of 8 KB for each of 8 warps are enough: a batch of 128 sequences
-//   up to 8191 keys takes 311 us (6.7 TB/s); with three stages, when it took 318, 341.
+//   up to 8191 keys takes 306 to 321 us on different boards, the copy rate; with
+//   three stages, when it took 318, 341.
 // * Two cursors walk over the tiles, one for copies and one for arithmetic, so
 //   that the copies run on across the ends of sequences and heads.
 //
@@ -71,7 +72,8 @@ struct Ring {
   static constexpr int kBytes = kStages * kStageBytes;  // of a warp
   static constexpr int kPitch = Policy::kDim + 4;       // of a merged row, in floats
   // A part put aside, in shared memory but for 16 rows of 256 columns, whose
-  // kernel needs what is left for L1 (16/1 heads of 256: 31.0 against 34.3 us).
+  // kernel spills and is slower with less L1 (16/1 heads of 256: 31.0 us, against
+  // 34.3 with the parts in shared memory).
   static constexpr bool kSharedHeads = Policy::kRows * Policy::kDim <= 16 * 192;
   static constexpr int kHeadBytes = kSharedHeads ? Policy::kRows * kPitch * 4 : 0;
   static constexpr size_t kShared =

@@ -10,7 +10,7 @@
 //
 // Angle: the product is formed in FP64, in turns, and its whole turns are
 // removed before anything is rounded to FP32 -- at position 10^6 an FP32
-// product is off by 0.06 radians.  The fraction, rounded once to FP32
+// product is off by up to 0.03 radians.  The fraction, rounded once to FP32
 // (relative 2^-24), goes through sincospif.
 //
 // Bound by HBM: every element is read and written once.  One warp owns a
