@@ -92,25 +92,30 @@ def attention_into(q, k, v, out, causal: bool, stream=None) -> None:
                            int(bool(causal)), _stream(q, stream)))
 
 
-def _require_rows(name, t, like, shape=None, written=False) -> None:
-    """A strided operand: like's dtype and device, the last dimension contiguous."""
-    if t.dtype != like.dtype or t.device != like.device:
+def _require_rows(name, t, dtype, device, shape=None, written=False) -> None:
+    """A strided operand: the last dimension contiguous, at least the first
+    dimension's rows."""
+    if t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must have the other tensors' dtype and device")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{name} must have the shape {list(shape)}")
+    own = t.shape
+    if shape is not None and own != shape and (len(own) != len(shape) or own[1:] != shape[1:]
+                                               or own[0] < shape[0]):
+        raise ValueError(f"{name} must have the shape {list(shape)}, or more rows")
     strides = t.stride()
-    if strides[-1] != 1 and t.shape[-1] != 1:
+    if strides[-1] != 1 and own[-1] != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
-    if written and 0 in strides and any(s == 0 and n > 1 for s, n in zip(strides, t.shape)):
+    if written and 0 in strides and any(s == 0 and n > 1 for s, n in zip(strides, own)):
         raise ValueError(f"{name} is written and must not be expanded")
 
 
-def _require_index(name, t, like, dtype, shape) -> None:
-    """Contiguous numbers that the kernel indexes by itself."""
-    if t.dtype != dtype or t.device != like.device:
+def _require_flat(name, t, dtype, device, count, exact=False) -> None:
+    """Contiguous numbers, at least (or exactly) `count`."""
+    if t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must be {str(dtype).split('.')[-1]} on the other tensors' device")
-    if t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous with the shape {list(shape)}")
+    size = t.numel()
+    if size < count or (exact and size != count) or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous with {'' if exact else 'at least '}{count} "
+                         "elements")
 
 
 def _require_dims(name, t, dims) -> None:
@@ -118,20 +123,19 @@ def _require_dims(name, t, dims) -> None:
         raise ValueError(f"{name} must have {dims} dimensions")
 
 
-def _rope_spec(x, positions, inv_freq, sections, adjacent, inverse):
+def _rope_spec(tokens, device, positions, inv_freq, sections, adjacent, inverse):
     import torch
 
     from . import RopeSpec
 
-    pairs, tokens = inv_freq.numel(), x.shape[0]
+    pairs = inv_freq.numel()
     sections = list(sections) if sections else [pairs]
     if len(sections) > 4:
         raise ValueError("a rotary embedding has at most 4 position axes")
-    _require_index("inv_freq", inv_freq, x, torch.float32, (pairs,))
-    # One axis may come as [tokens] or [1, tokens].
-    whole = len(sections) == 1 and positions.dim() == 1
-    _require_index("positions", positions, x, torch.int64,
-                   (tokens,) if whole else (len(sections), tokens))
+    _require_flat("inv_freq", inv_freq, torch.float32, device, pairs)
+    if pairs > 0:  # the kernel finds an axis at axis * tokens
+        _require_flat("positions", positions, torch.int64, device, len(sections) * tokens,
+                      exact=len(sections) > 1)
     spec = RopeSpec(positions=_ptr(positions), inv_freq=_ptr(inv_freq), rot_dim=2 * pairs,
                     axes=len(sections), adjacent=int(bool(adjacent)),
                     inverse=int(bool(inverse)))
@@ -139,18 +143,17 @@ def _rope_spec(x, positions, inv_freq, sections, adjacent, inverse):
     return spec
 
 
-def _kv_cache(q, k_cache, v_cache, written):
+def _kv_cache(q, dtype, device, k_cache, v_cache, written):
     from . import KvCache
 
     _require_dims("k_cache", k_cache, 4)
-    _require_rows("k_cache", k_cache, q, written=written)
-    _require_rows("v_cache", v_cache, q, k_cache.shape, written=written)
-    if k_cache.shape[3] != q.shape[2]:
+    shape = k_cache.shape
+    _require_rows("k_cache", k_cache, dtype, device, written=written)
+    _require_rows("v_cache", v_cache, dtype, device, shape, written)
+    if shape[3] != q.shape[2]:
         raise ValueError("the caches must be [pages, page_size, kv_heads, head_dim] with q's "
                          "head_dim")
-    pages, page_size, kv_heads, head_dim = k_cache.shape
-    return KvCache(_ptr(k_cache), _ptr(v_cache), pages, page_size, kv_heads, head_dim,
-                   *k_cache.stride()[:3], *v_cache.stride()[:3])
+    return KvCache(_ptr(k_cache), _ptr(v_cache), *shape, *k_cache.stride()[:3], *v_cache.stride()[:3])
 
 
 def rope_into(x, out, positions, inv_freq, sections=None, adjacent=False, inverse=False,
@@ -163,12 +166,13 @@ def rope_into(x, out, positions, inv_freq, sections=None, adjacent=False, invers
     import torch
 
     _require_dims("x", x, 3)
-    _require_rows("x", x, x)
-    _require_rows("out", out, x, x.shape, written=True)
-    tokens, heads, head_dim = x.shape
-    spec = _rope_spec(x, positions, inv_freq, sections, adjacent, inverse)
-    with torch.cuda.device(x.device):
-        _check("rope", _dtype_fn("rope", x.dtype)(
+    dtype, device, shape = x.dtype, x.device, x.shape
+    tokens, heads, head_dim = shape
+    _require_rows("x", x, dtype, device)
+    _require_rows("out", out, dtype, device, shape, True)
+    spec = _rope_spec(tokens, device, positions, inv_freq, sections, adjacent, inverse)
+    with torch.cuda.device(device):
+        _check("rope", _dtype_fn("rope", dtype)(
             _ptr(x), _ptr(out), tokens, heads, head_dim, *x.stride()[:2], *out.stride()[:2],
             ctypes.byref(spec), _stream(x, stream)))
 
@@ -184,19 +188,21 @@ def kv_append_into(q, k, v, q_out, k_cache, v_cache, slots, positions, inv_freq,
     import torch
 
     _require_dims("q", q, 3)
-    _require_rows("q", q, q)
-    _require_rows("q_out", q_out, q, q.shape, written=True)
-    cache = _kv_cache(q, k_cache, v_cache, written=True)
-    new = (q.shape[0], *k_cache.shape[2:])
-    _require_rows("k", k, q, new)
-    _require_rows("v", v, q, new)
-    _require_index("slots", slots, q, torch.int64, (q.shape[0],))
-    spec = _rope_spec(q, positions, inv_freq, sections, adjacent, False)
-    with torch.cuda.device(q.device):
-        _check("kv_append", _dtype_fn("kv_append", q.dtype)(
+    dtype, device, shape = q.dtype, q.device, q.shape
+    tokens, heads, head_dim = shape
+    _require_rows("q", q, dtype, device)
+    _require_rows("q_out", q_out, dtype, device, shape, True)
+    cache = _kv_cache(q, dtype, device, k_cache, v_cache, True)
+    new = (tokens, cache.kv_heads, head_dim)
+    _require_rows("k", k, dtype, device, new)
+    _require_rows("v", v, dtype, device, new)
+    _require_flat("slots", slots, torch.int64, device, tokens)
+    spec = _rope_spec(tokens, device, positions, inv_freq, sections, adjacent, False)
+    with torch.cuda.device(device):
+        _check("kv_append", _dtype_fn("kv_append", dtype)(
             _ptr(q), *q.stride()[:2], _ptr(k), *k.stride()[:2], _ptr(v), *v.stride()[:2],
-            _ptr(q_out), *q_out.stride()[:2], ctypes.byref(cache), _ptr(slots), q.shape[0],
-            q.shape[1], ctypes.byref(spec), _stream(q, stream)))
+            _ptr(q_out), *q_out.stride()[:2], ctypes.byref(cache), _ptr(slots), tokens,
+            heads, ctypes.byref(spec), _stream(q, stream)))
 
 
 def paged_attention_workspace(heads: int, kv_heads: int, head_dim: int, device) -> "torch.Tensor":
@@ -223,23 +229,25 @@ def paged_attention_into(q, k_cache, v_cache, block_table, seq_lens, out, worksp
     import torch
 
     _require_dims("q", q, 3)
-    _require_rows("q", q, q)
-    _require_index("out", out, q, q.dtype, q.shape)
-    cache = _kv_cache(q, k_cache, v_cache, written=False)
+    dtype, device = q.dtype, q.device
     batch, heads, head_dim = q.shape
+    _require_rows("q", q, dtype, device)
+    _require_flat("out", out, dtype, device, q.numel())
+    cache = _kv_cache(q, dtype, device, k_cache, v_cache, False)
     _require_dims("block_table", block_table, 2)
-    columns = block_table.shape[1]
-    if (block_table.dtype != torch.int32 or block_table.device != q.device
-            or block_table.shape[0] != batch or (block_table.stride(1) != 1 and columns != 1)):
+    rows, columns = block_table.shape
+    table_row, step = block_table.stride()
+    if (block_table.dtype != torch.int32 or block_table.device != device or rows < batch
+            or (step != 1 and columns != 1)):
         raise ValueError("block_table must be int32 [batch, pages] on the other tensors' device, "
                          "contiguous in its last dimension")
-    _require_index("seq_lens", seq_lens, q, torch.int32, (batch,))
-    if workspace.device != q.device or not workspace.is_contiguous():
+    _require_flat("seq_lens", seq_lens, torch.int32, device, batch)
+    if workspace.device != device or not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous on the other tensors' device")
     scale = head_dim ** -0.5 if scale is None else float(scale)
-    with torch.cuda.device(q.device):
-        _check("paged_attention", _dtype_fn("paged_attention", q.dtype)(
+    with torch.cuda.device(device):
+        _check("paged_attention", _dtype_fn("paged_attention", dtype)(
             _ptr(q), *q.stride()[:2], ctypes.byref(cache), _ptr(block_table),
-            block_table.stride(0), columns, _ptr(seq_lens), _ptr(out), batch, heads,
+            table_row, columns, _ptr(seq_lens), _ptr(out), batch, heads,
             scale, _ptr(workspace), workspace.numel() * workspace.element_size(),
             _stream(q, stream)))

@@ -41,8 +41,8 @@ def attention_args(**kw):
 
 
 ROPE = [
-    (dict(positions=t(4, dtype=I64)), "positions must be contiguous with the shape"),
-    (dict(positions=t(6, dtype=I64)), "positions must be contiguous with the shape"),
+    (dict(positions=t(4, dtype=I64)), "positions must be contiguous with at least 5"),
+    (dict(positions=t(3, 6, dtype=I64), sections=[16, 8, 8]), "positions must be .* with 15 elem"),
     (dict(positions=t(5, dtype=I32)), "positions must be int64"),
     (dict(positions=t(5, dtype=I64), sections=[16, 8, 8]), "positions must be contiguous"),
     (dict(positions=t(2, 5, dtype=I64), sections=[16, 8, 8]), "positions must be contiguous"),
@@ -50,7 +50,6 @@ ROPE = [
     (dict(positions=t(10, dtype=I64)[::2]), "positions must be contiguous"),
     (dict(inv_freq=t(32, dtype=torch.float64)), "inv_freq must be float32"),
     (dict(inv_freq=t(64, dtype=torch.float32)[::2]), "inv_freq must be contiguous"),
-    (dict(inv_freq=t(2, 16, dtype=torch.float32)), "inv_freq must be contiguous"),
 ]
 
 
@@ -80,7 +79,7 @@ def test_rope_into(change, text):
     (dict(k_cache=t(1, 16, 2, 64).expand(3, 16, 2, 64)), "k_cache is written"),
     (dict(k_cache=t(3, 16, 2, 32), v_cache=t(3, 16, 2, 32)), "with q's head_dim"),
     (dict(slots=t(5, dtype=I32)), "slots must be int64"),
-    (dict(slots=t(4, dtype=I64)), "slots must be contiguous with the shape"),
+    (dict(slots=t(4, dtype=I64)), "slots must be contiguous with at least 5"),
     (dict(slots=t(10, dtype=I64)[::2]), "slots must be contiguous"),
 ])
 def test_kv_append_into(change, text):
@@ -90,7 +89,7 @@ def test_kv_append_into(change, text):
 
 @pytest.mark.parametrize("change,text", [
     (dict(q=t(5, 256)), "q must have 3 dimensions"),
-    (dict(out=t(4, 4, 64)), "out must be contiguous with the shape"),
+    (dict(out=t(4, 4, 64)), "out must be contiguous with at least 1280"),
     (dict(out=t(5, 4, 128)[..., :64]), "out must be contiguous"),
     (dict(out=t(5, 4, 64, dtype=torch.float32)), "out must be float16"),
     (dict(v_cache=t(2, 16, 2, 64)), "v_cache must have the shape"),
@@ -101,7 +100,7 @@ def test_kv_append_into(change, text):
     (dict(block_table=t(2, 5, dtype=I32).t()), "contiguous in its last"),
     (dict(block_table=t(10, dtype=I32)), "block_table must have 2 dimensions"),
     (dict(seq_lens=t(5, dtype=I64)), "seq_lens must be int32"),
-    (dict(seq_lens=t(4, dtype=I32)), "seq_lens must be contiguous with the shape"),
+    (dict(seq_lens=t(4, dtype=I32)), "seq_lens must be contiguous with at least 5"),
     (dict(workspace=t(1 << 20, dtype=torch.uint8)[::2]), "workspace must be contiguous"),
     (dict(workspace=t(1 << 20, dtype=torch.uint8).to("meta")), "workspace must be"),
 ])
@@ -111,17 +110,23 @@ def test_paged_attention_into(change, text):
 
 
 def test_operands_that_go_together_are_not_refused():
-    """Past the checks, a CPU tensor is refused by the device guard."""
+    """Past the checks, a CPU tensor is refused by the device guard.  Buffers for
+    more tokens or sequences than the call has may be passed whole."""
     for call, args in ((operatorlib.rope_into, rope_args()),
                        (operatorlib.rope_into, rope_args(positions=t(1, 5, dtype=I64))),
                        (operatorlib.rope_into, rope_args(positions=t(3, 5, dtype=I64),
                                                          sections=[16, 8, 8])),
+                       (operatorlib.rope_into, rope_args(positions=t(9, dtype=I64),
+                                                         out=t(8, 3, 64))),
                        (operatorlib.rope_into, rope_args(
                            x=t(5, 9, 64)[:, 2:5], out=t(3, 5, 64).transpose(0, 1))),
                        (operatorlib.kv_append_into, append_args(
                            k_cache=t(3, 2, 16, 64).transpose(1, 2), k=t(5, 1, 64).expand(5, 2, 64))),
                        (operatorlib.paged_attention_into, attention_args(
-                           block_table=t(5, 9, dtype=I32)[:, 2:4]))):
+                           block_table=t(5, 9, dtype=I32)[:, 2:4])),
+                       (operatorlib.paged_attention_into, attention_args(
+                           block_table=t(7, 2, dtype=I32), seq_lens=t(7, dtype=I32),
+                           out=t(5, 256)))):
         with pytest.raises(ValueError, match="Expected a cuda device"):
             call(**args)
 
