@@ -14,7 +14,7 @@
 //   their issue alone bounds the kernel (106 us with no arithmetic, 138 us when
 //   a group of eight lanes does not cover 128 bytes of a row; TMA 87 us with it).
 // * Two stages of 8 KB for each of 8 warps are enough: a batch of 128 sequences
-//   up to 8191 keys takes 306 to 321 us on different boards, the copy rate; with
+//   up to 8191 keys takes 306 to 323 us on different boards, the copy rate; with
 //   three stages, when it took 318, 341.
 // * Two cursors walk over the tiles, one for copies and one for arithmetic, so
 //   that the copies run on across the ends of sequences and heads.
